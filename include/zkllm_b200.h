@@ -321,6 +321,99 @@ int zkb_softmax_shift(const zkb_fr_t* d_A, zkb_fr_t* d_shift, zkb_fr_t* d_out, s
 int zkb_softmax_decompose(const zkb_fr_t* d_X, const uint32_t* h_bs, unsigned K, zkb_fr_t* d_out,
                           size_t N, void* stream);
 
+/* ---- the float side of a layer -------------------------------------------------------
+ * The stages above work on fixed-point values; what those are made from - the norms' statistics, the turned queries and
+ * keys, the feed-forward block that a fixed-point one is calibrated to, and the gradients that fit the weights before they
+ * are fixed and committed - is float work.  These operators have no counterpart in the reference's C++ (its Python side
+ * computes them: llama-rmsnorm.py:37-39, llama-self-attn.py:48-65, llama-ffn.py:16-19).
+ *  - Tensors are device memory of the current device, of one type `dtype`; strides count elements, a row's values are
+ *    consecutive and every stride and address may be any multiple of the element size.  16-byte alignment of addresses
+ *    and strides is faster.  Host arrays and other devices' memory are refused.
+ *  - All sums, statistics and angles are held in 32 bits or more; a result is rounded once, to nearest even.
+ *  - Results do not depend on timing: the same call gives the same bits.
+ *  - Calls are asynchronous on `stream`, may be captured into a graph, and take their workspace from the library's pool
+ *    for each call, so that captured graphs share none.
+ *  - An output may be the memory of an input of the same shape and strides where that is said; otherwise memory of
+ *    outputs overlaps nothing. */
+#define ZKB_F32  0
+#define ZKB_F16  1
+#define ZKB_BF16 2
+
+/* Rotary positions (no counterpart in the reference's C++).  Pair i of a head at position p is turned by the angle
+ * p * inv_freq[i] and multiplied by `magnitude`;
+ * pairs are (x[i], x[i + rotary_dim/2]), or (x[2i], x[2i+1]) with interleaved != 0; the head_dim - rotary_dim values
+ * behind them are copied.  backward != 0 turns by the opposite angle: d_in is then the gradient of the output and d_out
+ * that of the input.  A call takes up to four tensors (queries, keys) of `batch` x `tokens` positions with their own numbers
+ * of heads and strides; d_out may be d_in where their strides agree.  Positions: d_positions[b * position_batch_stride + t],
+ * or first_position + t where d_positions is NULL; they may be negative and are exact up to 2^53.  d_inv_freq holds
+ * rotary_dim / 2 values on the device.  head_dim up to 8192. */
+typedef struct {
+    const void* d_in;
+    void* d_out;
+    size_t heads;
+    int64_t in_batch, in_token, in_head, out_batch, out_token, out_head;   /* strides, in elements */
+} zkb_rope_tensor_t;
+int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, size_t batch, size_t tokens, size_t head_dim,
+             size_t rotary_dim, int interleaved, const double* d_inv_freq, float magnitude, const int64_t* d_positions,
+             int64_t position_batch_stride, int64_t first_position, int backward, void* stream);
+/* The rotary_dim / 2 frequencies base^(-2i / rotary_dim) in radians a position, for a context stretched by `factor`
+ * (host arithmetic; no counterpart in the reference).  PLAIN: as they are; LINEAR: all divided by the factor; BASE: the base
+ * raised to base * factor^(n / (n - 2)), n = rotary_dim; RAMP: pairs that make more than fast_turns turns over original_len
+ * positions stay, those that make fewer than slow_turns are divided by the factor, with a linear ramp over the pairs
+ * between, and *h_magnitude is 0.1 ln(factor) + 1 (1 for the others). */
+#define ZKB_ROPE_PLAIN  0
+#define ZKB_ROPE_LINEAR 1
+#define ZKB_ROPE_BASE   2
+#define ZKB_ROPE_RAMP   3
+int zkb_rope_frequencies(int scaling, unsigned rotary_dim, double base, double factor, double original_len, double fast_turns,
+                         double slow_turns, double* h_inv_freq, float* h_magnitude);
+
+/* The norms after one branch of a layer and before the next, with the branch's gate, residual scale and addition between
+ * them (no counterpart in the reference's C++; its rmsnorm.cu:36-41 and skip-connection.cu:11-18 are the fixed-point forms):
+ *   n = y / sqrt(mean y^2 + eps) * post_gain     (post_norm == 0: n = y)
+ *   r = x + residual_scale * gate * n            (d_y NULL: r = x)
+ *   z = r / sqrt(mean r^2 + eps) * pre_gain      (pre_norm == 0: no z)
+ * over rows of `cols` values (up to 16384).  The gate is one value for each channel (CHANNEL, [cols]), for each row (ROW, [rows]) or
+ * for each value (ELEMENT, [rows, cols] with ldgate).  Gains and a CHANNEL gate are of gains_dtype: dtype or ZKB_F32; a NULL gain is
+ * ones.  d_r, d_z, d_post_inv and d_pre_inv may be NULL; the last two receive 1 / sqrt(mean + eps) of each row.  z is
+ * formed from r before r is rounded.  r and z may be x's, y's or an ELEMENT gate's memory. */
+#define ZKB_GATE_NONE    0
+#define ZKB_GATE_CHANNEL 1
+#define ZKB_GATE_ROW     2
+#define ZKB_GATE_ELEMENT 3
+int zkb_block_norm(int dtype, int gains_dtype, size_t rows, size_t cols, const void* d_x, size_t ldx, const void* d_y, size_t ldy,
+                   int post_norm, const void* d_post_gain, int gate_kind, const void* d_gate, size_t ldgate, float residual_scale,
+                   int pre_norm, const void* d_pre_gain, float eps, void* d_r, size_t ldr, void* d_z, size_t ldz,
+                   float* d_post_inv, float* d_pre_inv, void* stream);
+/* Its gradients (no counterpart in the reference).  d_r, d_y, the gains and the gate are the forward call's; d_dz is the gradient of z, d_dr
+ * the one that reaches r besides (NULL: none).  d_dx receives the gradient of x, which is the whole gradient of r; d_dy that of y;
+ * d_dgate the gate's, in the gate's shape and type; d_dpost_gain and d_dpre_gain [cols] the gains'.  Any output may be NULL.
+ * d_dx may be d_dr's memory or d_dz's, d_dy may be d_y's.  Zero rows give zero sums. */
+int zkb_block_norm_backward(int dtype, int gains_dtype, size_t rows, size_t cols, const void* d_r, size_t ldr, const void* d_y,
+                            size_t ldy, int post_norm, const void* d_post_gain, int gate_kind, const void* d_gate, size_t ldgate,
+                            float residual_scale, int pre_norm, const void* d_pre_gain, float eps, const void* d_dz, size_t lddz,
+                            const void* d_dr, size_t lddr, void* d_dx, size_t lddx, void* d_dy, size_t lddy, void* d_dgate,
+                            size_t lddgate, void* d_dpost_gain, void* d_dpre_gain, void* stream);
+
+/* The gated feed-forward block up to its product: h = act(x w_gate) * (x w_up), x [tokens, in_dim], both weights
+ * [in_dim, hidden] as zkFC takes them (zkfc.cu:44-58; ffn.cu:57-70 is the fixed-point form), f16 or bf16.  d_gate and d_up, both
+ * or none, receive the two projections for the gradients.  h is formed from the unrounded projections.
+ * GELU is the exact form, GELU_TANH the usual approximation. */
+#define ZKB_ACT_SILU      0
+#define ZKB_ACT_GELU      1
+#define ZKB_ACT_GELU_TANH 2
+#define ZKB_ACT_RELU      3
+int zkb_glu(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidden, const void* d_x, size_t ldx,
+            const void* d_w_gate, size_t ldwg, const void* d_w_up, size_t ldwu, void* d_h, size_t ldh, void* d_gate, size_t ldg,
+            void* d_up, size_t ldu, void* stream);
+/* Its gradients (no counterpart in the reference), from the two projections as zkb_glu kept them and the gradient of h:
+ * d_dx [tokens, in_dim] (or NULL), d_dw_gate and d_dw_up [in_dim, hidden] (or both NULL).  The gradients of the projections are
+ * rounded to the tensors' type before the products with the weights and with x. */
+int zkb_glu_backward(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidden, const void* d_x, size_t ldx,
+                     const void* d_w_gate, size_t ldwg, const void* d_w_up, size_t ldwu, const void* d_gate, size_t ldg,
+                     const void* d_up, size_t ldu, const void* d_dh, size_t lddh, void* d_dx, size_t lddx, void* d_dw_gate,
+                     size_t lddwg, void* d_dw_up, size_t lddwu, void* stream);
+
 /* ---- G1 tensors: fills, negation, elementwise and broadcast add/sub, affine lift
  *      (g1-tensor.cu:61-375) -------------------------------------------------------------- */
 int zkb_g1_fill(zkb_g1_t* d_out, const zkb_g1_t* h_val, size_t n, void* stream);

@@ -41,7 +41,35 @@ def lib() -> ctypes.CDLL:
         _lib = ctypes.CDLL(str(LIB_PATH))
         _lib.zkb_last_error.restype = ctypes.c_char_p
         _lib.zkb_launch_count.restype = ctypes.c_ulonglong
+        for name, types in _FLOAT_OPERATORS.items():
+            getattr(_lib, name).argtypes = [_CTYPES[t] for t in types.split()]
     return _lib
+
+
+# Argument types of the float operators, so that addresses and sizes may be given to call() as plain numbers
+# (p: address or None, n: size, i: int, u: unsigned, l: signed 64 bits, f / d: float / double).
+_CTYPES = {"p": ctypes.c_void_p, "n": ctypes.c_size_t, "i": ctypes.c_int, "u": ctypes.c_uint, "l": ctypes.c_int64, "f": ctypes.c_float,
+           "d": ctypes.c_double}
+_FLOAT_OPERATORS = {
+    "zkb_rope_frequencies": "i u d d d d d p p",
+    "zkb_rope": "i p u n n n n i p f p l l i p",
+    "zkb_block_norm": "i i n n p n p n i p i p n f i p f p n p n p p p",
+    "zkb_block_norm_backward": "i i n n p n p n i p i p n f i p f p n p n p n p n p n p p p",
+    "zkb_glu": "i i n n n p n p n p n p n p n p n p",
+    "zkb_glu_backward": "i i n n n p n p n p n p n p n p n p n p n p n p",
+}
+
+
+class RopeTensor(ctypes.Structure):
+    """zkb_rope_tensor_t: one tensor of a zkb_rope call"""
+    _fields_ = [("d_in", ctypes.c_void_p), ("d_out", ctypes.c_void_p), ("heads", ctypes.c_size_t)] + [
+        (f"{side}_{axis}", ctypes.c_int64) for side in ("in", "out") for axis in ("batch", "token", "head")]
+
+
+def rope_tensors(*tensors):
+    """The array of tensors that zkb_rope takes, each given as (address in, address out, heads, strides in, strides out)
+    with the strides of batch, token and head in elements."""
+    return (RopeTensor * len(tensors))(*(RopeTensor(i, o, h, *si, *so) for i, o, h, si, so in tensors))
 
 
 def exported_symbols_from_header() -> list:

@@ -1,5 +1,6 @@
 // Library plumbing: error text, device memory entry points, scratch pool.
 #include "common.cuh"
+#include "floatops.cuh"
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -67,6 +68,21 @@ int sm_count() {
         cached[dev] = n;
     }
     return cached[dev];
+}
+
+int check_device(const void* p, size_t align, const char* what) {
+    if (!p) return ZKB_OK;
+    if (!aligned_to(p, align)) return fail(ZKB_ERR_ARG, std::string(what) + ": address is not a multiple of the element size");
+    cudaPointerAttributes at;
+    int dev = 0;
+    ZKB_CUDA(cudaGetDevice(&dev));
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(ZKB_ERR_ARG, std::string(what) + ": not an address that the device knows");
+    }
+    if (at.type == cudaMemoryTypeUnregistered) return fail(ZKB_ERR_ARG, std::string(what) + ": pageable host memory");
+    if (at.type == cudaMemoryTypeDevice && at.device != dev) return fail(ZKB_ERR_ARG, std::string(what) + ": memory of another device");
+    return ZKB_OK;
 }
 
 static bool nvtx_enabled() {
