@@ -3,7 +3,7 @@
 // Weights are [in, hidden], as zkFC and FrTensor::matmul take them.  Sums are in 32 bits; h is formed from the unrounded sums.
 #include <algorithm>
 
-#include "floatops.cuh"
+#include "tensorcore.cuh"
 
 namespace zkb {
 namespace {
@@ -32,75 +32,256 @@ __device__ __forceinline__ float activate(int kind, float g, float* d) {
     return fmaxf(g, 0.0f);
 }
 
-constexpr int kTile = 64, kDepth = 16;
+// ---- the product kernel -----------------------------------------------------------------------------------------------------
+//
+// One persistent block per SM works through 128 x kCols tiles.  Warp 0 copies 64-deep slices of both operands into a ring in
+// shared memory, warp 1 issues the products (128 x kCols x 16 each) into one of two accumulators in tensor memory, warps 4 to 7 take the
+// other accumulator out, so that a tile's epilogue runs beside the next tile's products.
+enum Form {
+    kGated,    // A x; B the two weights side by side, kCols / 2 columns of each in a tile; result act(g) * u
+    kSummed,   // A dg then du; B w_gate then w_up: one sum over both; result dx
+    kPaired    // A x^T; B dg for the first half of the tiles, du for the second; results dw_gate and dw_up
+};
+constexpr int kRows = 128, kDepth = 64;
+constexpr int kProductThreads = 256;
+constexpr int kStageBytes = 32 * 80;   // an epilogue warp's 32 x 32 values on their way out, rows 80 bytes apart
 
-// One 64 x 64 tile of sum_s A_s[m, k] B_s[k, n], any strides; 256 threads with 4 x 4 values each.
-struct Product { const void *a, *b; size_t a_row, a_col, b_row, b_col; };
+struct ProductArgs {
+    CUtensorMap a[2], b[2];
+    unsigned m, n;               // of the result (kGated: hidden)
+    unsigned row_tiles, col_tiles, slices;   // tiles of a result, slices of 64 of one sum
+    void* out[3];                // kGated: h, gate, up (or null); kSummed: dx; kPaired: dw_gate, dw_up
+    size_t ld[3];
+    bool wide[3];                // 16-byte stores
+    int act;
+    int* flag;
+};
+
+template <int kCols> constexpr int kRing = kCols == 256 ? 4 : 3;
+template <int kCols> constexpr size_t product_smem() {
+    return 1024 + (size_t)kRing<kCols> * (kRows + kCols) * kDepth * 2 + 4 * kStageBytes + 256;
+}
+
+// 32 x 32 values of a warp (row i with lane i) to rows row0.. and columns col0.. of a matrix of m x n.
 template <class T>
-__device__ void tile_product(const Product& p, size_t M, size_t N, size_t K, float (&acc)[4][4]) {
-    __shared__ float as[kDepth][kTile + 1], bs[kDepth][kTile + 1];
-    const size_t m0 = (size_t)blockIdx.y * kTile, n0 = (size_t)blockIdx.x * kTile;
-    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    for (size_t k0 = 0; k0 < K; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-            const int m = p.a_col == 1 ? i / kDepth : i % kTile, k = p.a_col == 1 ? i % kDepth : i / kTile;
-            as[k][m] = m0 + m < M && k0 + k < K ? to_f32<T>(static_cast<const T*>(p.a)[(m0 + m) * p.a_row + (k0 + k) * p.a_col]) : 0.0f;
-            const int n = p.b_row == 1 ? i / kDepth : i % kTile, kb = p.b_row == 1 ? i % kDepth : i / kTile;
-            bs[kb][n] = n0 + n < N && k0 + kb < K ? to_f32<T>(static_cast<const T*>(p.b)[(k0 + kb) * p.b_row + (n0 + n) * p.b_col]) : 0.0f;
-        }
-        __syncthreads();
+__device__ __forceinline__ void store_block(char* stage, const float (&v)[32], T* out, size_t ld, bool wide, unsigned row0, unsigned col0, unsigned m,
+                                            unsigned n) {
+    const unsigned lane = threadIdx.x & 31;
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k)
+    for (int i = 0; i < 32; i += 8) {
+        Vec<T, 8> x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty + 16 * i] * bs[k][tx + 16 * j];
-        __syncthreads();
+        for (int j = 0; j < 8; ++j) x.v[j] = from_f32<T>(v[i + j]);
+        *reinterpret_cast<Vec<T, 8>*>(stage + lane * 80 + i * 2) = x;
     }
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned r = i * 8 + lane / 4, c = (lane % 4) * 8;
+            const Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8>*>(stage + r * 80 + c * 2);
+            if (row0 + r >= m) continue;
+            T* to = out + (size_t)(row0 + r) * ld + col0 + c;
+            if (col0 + c + 8 <= n) {
+                *reinterpret_cast<Vec<T, 8>*>(to) = x;
+            } else {
+                for (unsigned j = 0; col0 + c + j < n && j < 8; ++j) to[j] = x.v[j];
+            }
+        }
+    } else {
+        for (unsigned r = 0; r < 32 && row0 + r < m; ++r)
+            if (col0 + lane < n) out[(size_t)(row0 + r) * ld + col0 + lane] = *reinterpret_cast<const T*>(stage + r * 80 + lane * 2);
+    }
+    __syncwarp();
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) glu_kernel(Product pg, Product pu, size_t M, size_t N, size_t K, T* h, size_t ldh, T* gate, size_t ldg, T* up,
-                                                  size_t ldu, int act) {
-    float g[4][4] = {}, u[4][4] = {};
-    tile_product<T>(pg, M, N, K, g);
-    tile_product<T>(pu, M, N, K, u);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const size_t m = (size_t)blockIdx.y * kTile + threadIdx.x / 16 + 16 * i, n = (size_t)blockIdx.x * kTile + threadIdx.x % 16 + 16 * j;
-            if (m >= M || n >= N) continue;
-            h[m * ldh + n] = from_f32<T>(activate<false>(act, g[i][j], nullptr) * u[i][j]);
-            if (gate) gate[m * ldg + n] = from_f32<T>(g[i][j]);
-            if (up) up[m * ldu + n] = from_f32<T>(u[i][j]);
-        }
+// Tile number to its row and column: rows first within bands of 16 rows of tiles, so that the blocks at work at one time share
+// both operands in L2.
+__device__ __forceinline__ void tile_place(unsigned tile, unsigned row_tiles, unsigned col_tiles, unsigned* row, unsigned* col) {
+    const unsigned band = tile / (16 * col_tiles), in = tile % (16 * col_tiles);
+    const unsigned height = min(16u, row_tiles - band * 16);
+    *row = band * 16 + in % height;
+    *col = in / height;
 }
 
-// one product, or the sum of two
-template <class T>
-__global__ void __launch_bounds__(256) glu_product_kernel(Product p0, Product p1, int products, size_t M, size_t N, size_t K, T* c, size_t ldc) {
-    float acc[4][4] = {};
-    tile_product<T>(p0, M, N, K, acc);
-    if (products == 2) tile_product<T>(p1, M, N, K, acc);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const size_t m = (size_t)blockIdx.y * kTile + threadIdx.x / 16 + 16 * i, n = (size_t)blockIdx.x * kTile + threadIdx.x % 16 + 16 * j;
-            if (m < M && n < N) c[m * ldc + n] = from_f32<T>(acc[i][j]);
+template <class T, int kForm, int kCols>
+__global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __grid_constant__ ProductArgs p) {
+    constexpr bool kAMn = kForm == kPaired, kBMn = kForm != kSummed;
+    constexpr int kA = kRows * kDepth * 2, kB = kCols * kDepth * 2, kSlice = kA + kB, kR = kRing<kCols>;
+    constexpr uint32_t kInstruction = tc::instruction<T>(kRows, kCols, kAMn, kBMn);
+    constexpr int kSums = kForm == kSummed ? 2 : 1;
+    extern __shared__ char raw[];
+    char* ring = raw + ((1024 - (tc::smem_address(raw) & 1023)) & 1023);
+    char* stages = ring + kR * kSlice;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stages + 4 * kStageBytes);
+    volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kR + 5);
+    const uint32_t full = tc::smem_address(bars), empty = full + 8 * kR, ready = empty + 8 * kR, taken = ready + 16, drained = taken + 16;
+    const uint32_t tmem_at = drained + 16;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const tc::Watch watch = {dead, p.flag};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kR; ++i) {
+            tc::barrier_init(full + 8 * i, 1);
+            tc::barrier_init(empty + 8 * i, 1);
         }
+        for (int i = 0; i < 2; ++i) {
+            tc::barrier_init(ready + 8 * i, 1);
+            tc::barrier_init(taken + 8 * i, 4);
+        }
+        tc::barrier_init(drained, 1);
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc::prefetch_map(&p.a[0]);
+        tc::prefetch_map(&p.b[0]);
+    }
+    if (warp == 2) tc::tmem_alloc(tmem_at, 2 * kCols);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
+
+    const unsigned tiles = p.row_tiles * p.col_tiles, all = kForm == kPaired ? 2 * tiles : tiles;
+    const unsigned slices = p.slices * kSums;
+    if (warp == 0 && lane == 0) {
+        unsigned at = 0, issued = 0;
+        uint32_t phase = 0;
+        bool fine = true;
+        for (unsigned t = blockIdx.x; t < all && fine; t += gridDim.x) {
+            unsigned row, col;
+            tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
+            const unsigned pair = t / tiles;
+            for (unsigned s = 0; s < slices; ++s) {
+                if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
+                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = full + 8 * at;
+                tc::barrier_expect(bar, kSlice);
+                ++issued;
+                const int sum = kForm == kSummed ? (int)(s / p.slices) : 0;
+                const int k = (int)(s - sum * p.slices) * kDepth;
+                if constexpr (kAMn) {
+                    for (int i = 0; i < kRows / 64; ++i) tc::load_box(&p.a[0], a + i * 8192, bar, row * kRows + i * 64, k);
+                } else {
+                    tc::load_box(&p.a[sum], a, bar, k, row * kRows);
+                }
+                if constexpr (kForm == kGated) {
+                    for (int i = 0; i < kCols / 128; ++i) {
+                        tc::load_box(&p.b[0], b + i * 8192, bar, col * (kCols / 2) + i * 64, k);
+                        tc::load_box(&p.b[1], b + (kCols / 128 + i) * 8192, bar, col * (kCols / 2) + i * 64, k);
+                    }
+                } else if constexpr (kForm == kPaired) {
+                    for (int i = 0; i < kCols / 64; ++i) tc::load_box(&p.b[pair], b + i * 8192, bar, col * kCols + i * 64, k);
+                } else {
+                    tc::load_box(&p.b[sum], b, bar, k, col * kCols);
+                }
+                if (++at == kR) { at = 0; phase ^= 1; }
+            }
+        }
+        if (!fine)   // the copies in flight write to this block's memory: it ends after them
+            for (unsigned i = issued > kR ? issued - kR : 0; i < issued; ++i) tc::barrier_wait(full + 8 * (i % kR), (i / kR) & 1, watch, true);
+    } else if (warp == 1 && lane == 0) {
+        unsigned at = 0, count = 0;
+        uint32_t phase = 0;
+        bool fine = true;
+        for (unsigned t = blockIdx.x; t < all && fine; t += gridDim.x, ++count) {
+            const unsigned acc = count & 1;
+            if (!tc::barrier_wait(taken + 8 * acc, ((count >> 1) & 1) ^ 1, watch)) { fine = false; break; }
+            tc::fence_after_sync();
+            for (unsigned s = 0; s < slices; ++s) {
+                if (!tc::barrier_wait(full + 8 * at, phase, watch)) { fine = false; break; }
+                tc::fence_after_sync();
+                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA;
+#pragma unroll
+                for (int k = 0; k < kDepth / 16; ++k)
+                    tc::product(tmem + acc * kCols, tc::tile_descriptor(a + k * (kAMn ? 2048 : 32), kAMn, 8192),
+                                tc::tile_descriptor(b + k * (kBMn ? 2048 : 32), kBMn, 8192), kInstruction, s || k);
+                tc::commit(empty + 8 * at);
+                if (++at == kR) { at = 0; phase ^= 1; }
+            }
+            if (fine) tc::commit(ready + 8 * acc);
+        }
+        if (!fine) {   // products in flight read this block's memory
+            tc::commit(drained);
+            tc::barrier_wait(drained, 0, watch, true);
+        }
+    } else if (warp >= 4) {
+        char* stage = stages + (warp - 4) * kStageBytes;
+        unsigned count = 0;
+        for (unsigned t = blockIdx.x; t < all; t += gridDim.x, ++count) {
+            unsigned row, col;
+            tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
+            const unsigned acc = count & 1, pair = t / tiles;
+            const bool fine = tc::barrier_wait(ready + 8 * acc, (count >> 1) & 1, watch);
+            if (!__all_sync(0xffffffffu, fine)) break;
+            tc::fence_after_sync();
+            const uint32_t from = tmem + ((warp - 4) * 32 << 16) + acc * kCols;
+            const unsigned row0 = row * kRows + (warp - 4) * 32;
+            if constexpr (kForm == kGated) {
+                for (int c = 0; c < kCols / 2; c += 32) {
+                    float g[32], u[32];
+                    tc::load_columns(from + c, g);
+                    tc::load_columns(from + kCols / 2 + c, u);
+                    const unsigned col0 = col * (kCols / 2) + c;
+                    if (p.out[1]) {
+                        store_block<T>(stage, g, static_cast<T*>(p.out[1]), p.ld[1], p.wide[1], row0, col0, p.m, p.n);
+                        store_block<T>(stage, u, static_cast<T*>(p.out[2]), p.ld[2], p.wide[2], row0, col0, p.m, p.n);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) g[i] = activate<false>(p.act, g[i], nullptr) * u[i];
+                    store_block<T>(stage, g, static_cast<T*>(p.out[0]), p.ld[0], p.wide[0], row0, col0, p.m, p.n);
+                }
+            } else {
+                for (int c = 0; c < kCols; c += 32) {
+                    float v[32];
+                    tc::load_columns(from + c, v);
+                    store_block<T>(stage, v, static_cast<T*>(p.out[pair]), p.ld[pair], p.wide[pair], row0, col * kCols + c, p.m, p.n);
+                }
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive(taken + 8 * acc);
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 2) {
+        tc::fence_after_sync();
+        tc::tmem_free(tmem, 2 * kCols);
+    }
 }
 
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
 // follow have to be: each is off by half a step at most, independently, so a sum over them is off by no more, relative to its
 // norm, than its own rounding.
-template <class T>
-__global__ void __launch_bounds__(256) glu_split_kernel(const T* gate, size_t ldg, const T* up, size_t ldu, const T* dh, size_t ldh, T* dg, T* du, size_t ld,
-                                                        size_t rows, size_t cols, int act) {
-    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * cols; i += (size_t)gridDim.x * 256) {
-        const size_t m = i / cols, n = i % cols;
-        const float g = to_f32<T>(gate[m * ldg + n]), u = to_f32<T>(up[m * ldu + n]), d = to_f32<T>(dh[m * ldh + n]);
-        float da;
-        const float a = activate<true>(act, g, &da);
-        dg[m * ld + n] = from_f32<T>(d * u * da);
-        du[m * ld + n] = from_f32<T>(d * a);
+template <class T, int V>
+__global__ void __launch_bounds__(256) glu_split_kernel(const T* __restrict__ gate, size_t ldg, const T* __restrict__ up, size_t ldu, const T* __restrict__ dh,
+                                                        size_t ldh, T* __restrict__ dg, T* __restrict__ du, size_t ld, size_t rows, size_t cols, int act) {
+    const size_t vecs = ld / 8;
+    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
+        const size_t m = i / vecs, n = i % vecs * 8;
+        float g[8], u[8], d[8];
+        if (V == 8 && n + 8 <= cols) {
+            load_vec<T, 8>(gate + m * ldg + n, g);
+            load_vec<T, 8>(up + m * ldu + n, u);
+            load_vec<T, 8>(dh + m * ldh + n, d);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool in = n + j < cols;
+                g[j] = in ? to_f32<T>(gate[m * ldg + n + j]) : 0.0f;
+                u[j] = in ? to_f32<T>(up[m * ldu + n + j]) : 0.0f;
+                d[j] = in ? to_f32<T>(dh[m * ldh + n + j]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float da;
+            const float a = activate<true>(act, g[j], &da);
+            g[j] = d[j] * u[j] * da;
+            u[j] = d[j] * a;
+        }
+        store_vec<T, 8>(dg + m * ld + n, g);
+        store_vec<T, 8>(du + m * ld + n, u);
     }
 }
 
@@ -113,35 +294,126 @@ struct GluArgs {
     size_t ldh, lddx, lddwg, lddwu;
 };
 
+// Rows that a tensor copy cannot read (an address or a stride that is no multiple of 16 bytes), laid out anew with a stride of
+// whole 16 bytes: one pass over the operand before the products.
+template <class T>
+__global__ void __launch_bounds__(256) glu_align_kernel(const T* __restrict__ from, size_t ld_from, T* __restrict__ to, size_t ld_to, size_t rows, size_t cols) {
+    const size_t vecs = ld_to / 8;
+    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / vecs, c = (i % vecs) * 8;
+        Vec<T, 8> x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.v[j] = c + j < cols ? from[r * ld_from + c + j] : from_f32<T>(0.0f);
+        *reinterpret_cast<Vec<T, 8>*>(to + r * ld_to + c) = x;
+    }
+}
+
+struct Operand { const void* p; size_t ld; };
+bool copyable(const void* p, size_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+template <class T>
+int align(Operand* x, size_t rows, size_t cols, Scratch* scratch, cudaStream_t s) {
+    const size_t ld = (cols + 7) / 8 * 8;
+    if (rows == 1) x->ld = ld;   // never used
+    if (copyable(x->p, x->ld)) return ZKB_OK;
+    T* to = scratch->get_n<T>(rows * ld);
+    if (!to) return ZKB_ERR_CUDA;
+    const auto glu_align = glu_align_kernel<T>;
+    ZKB_LAUNCH(glu_align, (unsigned)std::min<size_t>((rows * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(x->p), x->ld, to, ld, rows,
+               cols);
+    *x = {to, ld};
+    return ZKB_OK;
+}
+
+template <class T, int kForm, int kCols>
+int product_launch(const ProductArgs& p, cudaStream_t s) {
+    const auto glu_product = glu_product_kernel<T, kForm, kCols>;
+    constexpr size_t smem = product_smem<kCols>();
+    ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const unsigned tiles = p.row_tiles * p.col_tiles * (kForm == kPaired ? 2 : 1);
+    ZKB_LAUNCH(glu_product, std::min(tiles, (kCols == 256 ? 1u : 2u) * sm_count()), kProductThreads, smem, s, p);
+    return ZKB_OK;
+}
+
+template <class T> constexpr int kCode = std::is_same<T, __half>::value ? ZKB_F16 : ZKB_BF16;
+
+template <class T, int kCols>
+int glu_forward(const GluArgs& a, Operand x, Operand wg, Operand wu, ProductArgs& p, cudaStream_t s) {
+    ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kRows));
+    ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
+    ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
+    p.row_tiles = div_up(a.tokens, kRows), p.col_tiles = div_up(a.hidden, kCols / 2);
+    return product_launch<T, kGated, kCols>(p, s);
+}
+
 template <class T>
 int glu_launch(const GluArgs& a, cudaStream_t s) {
-    const auto glu = glu_kernel<T>;
-    ZKB_LAUNCH(glu, dim3(div_up(a.hidden, kTile), div_up(a.tokens, kTile)), 256, 0, s, Product{a.x, a.wg, a.ldx, 1, a.ldwg, 1},
-               Product{a.x, a.wu, a.ldx, 1, a.ldwu, 1}, a.tokens, a.hidden, a.in, static_cast<T*>(a.h), a.ldh, static_cast<T*>(a.gate_out), a.ldg,
-               static_cast<T*>(a.up_out), a.ldu, a.act);
-    return ZKB_OK;
+    if (!a.in) {   // a sum over nothing
+        for (auto [p, ld] : {Operand{a.h, a.ldh}, Operand{a.gate_out, a.ldg}, Operand{a.up_out, a.ldu}})
+            if (p) ZKB_CUDA(cudaMemset2DAsync(const_cast<void*>(p), ld * 2, 0, a.hidden * 2, a.tokens, s));
+        return ZKB_OK;
+    }
+    Scratch scratch(s);
+    Operand x = {a.x, a.ldx}, wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
+    ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
+    ZKB_TRY(align<T>(&wg, a.in, a.hidden, &scratch, s));
+    ZKB_TRY(align<T>(&wu, a.in, a.hidden, &scratch, s));
+    ProductArgs p = {};
+    p.m = (unsigned)a.tokens, p.n = (unsigned)a.hidden, p.slices = div_up(a.in, kDepth);
+    p.out[0] = a.h, p.out[1] = a.gate_out, p.out[2] = a.up_out;
+    p.ld[0] = a.ldh, p.ld[1] = a.ldg, p.ld[2] = a.ldu;
+    for (int i = 0; i < 3; ++i) p.wide[i] = copyable(p.out[i], p.ld[i]);
+    p.act = a.act;
+    p.flag = tc::wait_flag();
+    if (!p.flag) return ZKB_ERR_CUDA;
+    // few tiles: narrower ones, two blocks to an SM, so that more SMs read the weights
+    if ((size_t)div_up(a.tokens, kRows) * div_up(a.hidden, 128) < (size_t)sm_count()) return glu_forward<T, 128>(a, x, wg, wu, p, s);
+    return glu_forward<T, 256>(a, x, wg, wu, p, s);
 }
 
 template <class T>
 int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
+    const size_t F = a.hidden, ld = (F + 7) / 8 * 8;
+    if (!F || !a.tokens) {   // sums over nothing
+        if (a.dx && a.tokens) ZKB_CUDA(cudaMemset2DAsync(a.dx, a.lddx * 2, 0, a.in * 2, a.tokens, s));
+        if (a.dwg && F) ZKB_CUDA(cudaMemset2DAsync(a.dwg, a.lddwg * 2, 0, F * 2, a.in, s));
+        if (a.dwu && F) ZKB_CUDA(cudaMemset2DAsync(a.dwu, a.lddwu * 2, 0, F * 2, a.in, s));
+        return ZKB_OK;
+    }
+    if (!a.dx && !a.dwg) return ZKB_OK;
     Scratch scratch(s);
-    T* dg = scratch.get_n<T>(a.tokens * a.hidden);
-    T* du = scratch.get_n<T>(a.tokens * a.hidden);
+    T* dg = scratch.get_n<T>(a.tokens * ld);
+    T* du = scratch.get_n<T>(a.tokens * ld);
     if (!dg || !du) return ZKB_ERR_CUDA;
-    const auto glu_split = glu_split_kernel<T>;
-    const auto glu_product = glu_product_kernel<T>;
-    const size_t F = a.hidden;
-    if (a.tokens && F)
-        ZKB_LAUNCH(glu_split, (unsigned)std::min<size_t>(div_up(a.tokens * F, 256), 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
-                   static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, F, a.tokens, F, a.act);
-    if (a.dx && a.tokens)
-        ZKB_LAUNCH(glu_product, dim3(div_up(a.in, kTile), div_up(a.tokens, kTile)), 256, 0, s, Product{dg, a.wg, F, 1, 1, a.ldwg},
-                   Product{du, a.wu, F, 1, 1, a.ldwu}, 2, a.tokens, a.in, F, static_cast<T*>(a.dx), a.lddx);
-    for (int k = 0; k < 2; ++k) {
-        void* out = k ? a.dwu : a.dwg;
-        if (!out || !F) continue;
-        ZKB_LAUNCH(glu_product, dim3(div_up(F, kTile), div_up(a.in, kTile)), 256, 0, s, Product{a.x, k ? du : dg, 1, a.ldx, F, 1}, Product{}, 1, a.in, F,
-                   a.tokens, static_cast<T*>(out), k ? a.lddwu : a.lddwg);
+    const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, 8> : glu_split_kernel<T, 1>;
+    ZKB_LAUNCH(glu_split, (unsigned)std::min<size_t>((a.tokens * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
+               static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld, a.tokens, F, a.act);
+    ProductArgs p = {};
+    p.flag = tc::wait_flag();
+    if (!p.flag) return ZKB_ERR_CUDA;
+    if (a.dx) {
+        Operand wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
+        ZKB_TRY(align<T>(&wg, a.in, F, &scratch, s));
+        ZKB_TRY(align<T>(&wu, a.in, F, &scratch, s));
+        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, dg, a.tokens, F, ld, kRows));
+        ZKB_TRY(tc::make_map(&p.a[1], kCode<T>, du, a.tokens, F, ld, kRows));
+        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, F, wg.ld, 256));
+        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, F, wu.ld, 256));
+        p.m = (unsigned)a.tokens, p.n = (unsigned)a.in, p.slices = div_up(F, kDepth);
+        p.row_tiles = div_up(p.m, kRows), p.col_tiles = div_up(p.n, 256);
+        p.out[0] = a.dx, p.ld[0] = a.lddx, p.wide[0] = copyable(a.dx, a.lddx);
+        ZKB_TRY((product_launch<T, kSummed, 256>(p, s)));
+    }
+    if (a.dwg) {
+        Operand x = {a.x, a.ldx};
+        ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
+        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kDepth));
+        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
+        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, du, a.tokens, F, ld, kDepth));
+        p.m = (unsigned)a.in, p.n = (unsigned)F, p.slices = div_up(a.tokens, kDepth);
+        p.row_tiles = div_up(p.m, kRows), p.col_tiles = div_up(p.n, 256);
+        p.out[0] = a.dwg, p.ld[0] = a.lddwg, p.wide[0] = copyable(a.dwg, a.lddwg);
+        p.out[1] = a.dwu, p.ld[1] = a.lddwu, p.wide[1] = copyable(a.dwu, a.lddwu);
+        ZKB_TRY((product_launch<T, kPaired, 256>(p, s)));
     }
     return ZKB_OK;
 }
@@ -162,6 +434,57 @@ int check_common(const char* who, int dtype, int act, const GluArgs& a) {
 }
 
 }  // namespace
+
+namespace tc {
+
+static int* g_wait_flag = nullptr;
+static std::mutex g_wait_mutex;
+
+int* wait_flag() {
+    std::lock_guard<std::mutex> lock(g_wait_mutex);
+    if (!g_wait_flag) {
+        // the first call may be inside another stream's capture, which forbids allocations by default
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
+            cuda_fail(e, "cudaHostAlloc(wait flag)");
+            return nullptr;
+        }
+        *static_cast<volatile int*>(p) = 0;
+        g_wait_flag = static_cast<int*>(p);
+    }
+    return g_wait_flag;
+}
+int check_wait_flag(const char* who) {
+    std::lock_guard<std::mutex> lock(g_wait_mutex);
+    volatile int* f = g_wait_flag;
+    if (!f || !*f) return ZKB_OK;
+    *f = 0;
+    return fail(ZKB_ERR_CUDA, std::string(who) + ": a wait of an earlier call ran out, its results are incomplete");
+}
+
+int make_map(CUtensorMap* map, int dtype, const void* p, size_t rows, size_t cols, size_t ld, unsigned box_rows) {
+    static std::atomic<void*> entry{nullptr};
+    void* fn = entry.load();
+    if (!fn) {
+        cudaDriverEntryPointQueryResult found;
+        ZKB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (!fn || found != cudaDriverEntryPointSuccess) return fail(ZKB_ERR_CUDA, "tensor copies: the driver has no cuTensorMapEncodeTiled");
+        entry.store(fn);
+    }
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+    const cuuint32_t box[2] = {64, box_rows}, steps[2] = {1, 1};
+    const CUresult e = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn)(
+        map, dtype == ZKB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, steps,
+        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) return fail(ZKB_ERR_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string((int)e));
+    return ZKB_OK;
+}
+
+}  // namespace tc
 }  // namespace zkb
 
 using namespace zkb;
@@ -178,6 +501,7 @@ int zkb_glu(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidd
     a.x = d_x, a.ldx = ldx, a.wg = d_w_gate, a.ldwg = ldwg, a.wu = d_w_up, a.ldwu = ldwu;
     a.h = d_h, a.ldh = ldh, a.gate_out = d_gate, a.ldg = ldg, a.up_out = d_up, a.ldu = ldu;
     ZKB_TRY(check_common(who, dtype, activation, a));
+    ZKB_TRY(tc::check_wait_flag(who));
     if (!d_gate != !d_up) return fail(ZKB_ERR_ARG, "zkb_glu: gate and up are kept together or not at all");
     if (!tokens || !hidden) return ZKB_OK;
     ZKB_TRY(check_matrix(who, "x", d_x, tokens, in_dim, ldx, in_dim != 0));
@@ -202,6 +526,7 @@ int zkb_glu_backward(int dtype, int activation, size_t tokens, size_t in_dim, si
     a.gate = d_gate, a.ldg = ldg, a.up = d_up, a.ldu = ldu, a.dh = d_dh, a.lddh = lddh;
     a.dx = d_dx, a.lddx = lddx, a.dwg = d_dw_gate, a.lddwg = lddwg, a.dwu = d_dw_up, a.lddwu = lddwu;
     ZKB_TRY(check_common(who, dtype, activation, a));
+    ZKB_TRY(tc::check_wait_flag(who));
     if (!d_dw_gate != !d_dw_up) return fail(ZKB_ERR_ARG, "zkb_glu_backward: both weights' gradients or none");
     if (!in_dim) return ZKB_OK;
     const bool some = tokens && hidden;
