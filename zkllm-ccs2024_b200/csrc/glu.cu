@@ -252,132 +252,163 @@ __global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __gr
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------------
 //
-// Bound by the one read of both weights.  The weights are the 128-row operand here (64 columns of w_gate and the same 64 of w_up), the
-// tokens the narrow one, so that a slice in flight is nearly all weights; and the sum over in_dim is split over the blocks of a
-// cluster, so that every SM has three blocks' rings in flight.  Each block leaves its share of the 2 x 64 x kTokens sums in its own shared
-// memory, and after a cluster barrier each adds up and finishes 64 / cluster columns, shares in the order of their blocks.
-template <int kTokens> constexpr int kFewRing = kTokens == 16 ? 4 : 3;
-template <int kTokens> constexpr int kFewPerSm = kTokens <= 64 ? 3 : 2;
-template <int kTokens> constexpr size_t few_smem() { return 1024 + (size_t)kFewRing<kTokens> * (kRows + kTokens) * kDepth * 2 + 128; }
+// Bound by the one read of both weights.  The weights are the 128-row operand here (128 columns of each to a tile) and the tokens the
+// narrow one, so that a slice in flight is nearly all weights.  The slices of all tiles, in order, are dealt out evenly: one
+// block per SM takes a run of them, whole tiles or parts of tiles, through one ring that never drains, and leaves the sums of each
+// (part of a) tile in the workspace; glu_few_finish_kernel adds the parts of a tile, in order, and applies the activation.
+// Parts of a cluster that share a tile through distributed shared memory were measured before: no more than one such block ran on an
+// SM, and the ring of 72 KB that left to each read 4.0 TB/s.
+constexpr int kFewCols = 128;
+template <int kTokens> constexpr int kFewSlice = (2 * kFewCols + kTokens) * kDepth * 2;
+template <int kTokens> constexpr int kFewRing = kTokens <= 32 ? 6 : kTokens == 64 ? 5 : 4;
+template <int kTokens> constexpr size_t few_smem() { return 1024 + (size_t)kFewRing<kTokens> * kFewSlice<kTokens> + 256; }
 
 struct FewArgs {
     CUtensorMap x, w[2];
-    unsigned tokens, hidden, slices, blocks_per_tile;
+    unsigned tokens, tiles, slices;   // slices: of a tile
+    float* parts;                     // [tile + block][token][gate, up][128]
+    int* flag;
+};
+struct FewEnd {
+    const float* parts;
+    unsigned tokens, hidden, tiles, slices, blocks;
     void* out[3];
     size_t ld[3];
     int act;
-    int* flag;
 };
-
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
+// the first slice of a block's run
+__host__ __device__ __forceinline__ unsigned run_start(unsigned block, unsigned blocks, unsigned total) {
+    return (unsigned)((unsigned long long)total * block / blocks);
 }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ float cluster_load(uint32_t address, unsigned rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(address), "r"(rank) : "memory");
-    return v;
+// the block whose run holds a slice
+__device__ __forceinline__ unsigned run_of(unsigned slice, unsigned blocks, unsigned total) {
+    return (unsigned)((((unsigned long long)slice + 1) * blocks - 1) / total);
 }
 
 template <class T, int kTokens>
-__global__ void __launch_bounds__(128) glu_few_kernel(const __grid_constant__ FewArgs p) {
-    constexpr int kA = kRows * kDepth * 2, kB = kTokens * kDepth * 2, kSlice = kA + kB, kR = kFewRing<kTokens>;
-    constexpr uint32_t kInstruction = tc::instruction<T>(kRows, kTokens, true, false);
-    constexpr uint32_t kTmem = kTokens < 32 ? 32 : kTokens;
+__global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_constant__ FewArgs p) {
+    constexpr int kA = kFewCols * kDepth * 2, kSlice = kFewSlice<kTokens>, kR = kFewRing<kTokens>;
+    constexpr uint32_t kInstruction = tc::instruction<T>(kFewCols, kTokens, true, false);
+    constexpr uint32_t kAcc = 2 * kTokens;
     extern __shared__ char raw[];
     char* ring = raw + ((1024 - (tc::smem_address(raw) & 1023)) & 1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kR * kSlice);
-    const uint32_t full = tc::smem_address(bars), empty = full + 8 * kR, ready = empty + 8 * kR;
-    const uint32_t tmem_at = ready + 8;
-    volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kR + 2);
+    volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kR + 5);
+    const uint32_t full = tc::smem_address(bars), empty = full + 8 * kR, ready = empty + 8 * kR, taken = ready + 16, drained = taken + 16;
+    const uint32_t tmem_at = drained + 16;
     const tc::Watch watch = {dead, p.flag};
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned rank = cluster_rank(), parts = p.blocks_per_tile, tile = blockIdx.x / parts;
-    const unsigned first = p.slices * rank / parts, last = p.slices * (rank + 1) / parts;   // parts <= slices: none is empty
+    const unsigned total = p.tiles * p.slices, first = run_start(blockIdx.x, gridDim.x, total), last = run_start(blockIdx.x + 1, gridDim.x, total);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kR; ++i) {
             tc::barrier_init(full + 8 * i, 1);
             tc::barrier_init(empty + 8 * i, 1);
         }
-        tc::barrier_init(ready, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc::barrier_init(ready + 8 * i, 1);
+            tc::barrier_init(taken + 8 * i, 4);
+        }
+        tc::barrier_init(drained, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 2) tc::tmem_alloc(tmem_at, kTmem);
+    if (warp == 2) tc::tmem_alloc(tmem_at, 2 * kAcc);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 1);
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
 
     if (warp == 0 && lane == 0) {
         unsigned issued = 0;
         bool fine = true;
         for (unsigned s = first; s < last; ++s, ++issued) {
-            const unsigned at = issued % kR;
+            const unsigned at = issued % kR, col = s / p.slices * kFewCols, k = s % p.slices * kDepth;
             if (!tc::barrier_wait(empty + 8 * at, ((issued / kR) & 1) ^ 1, watch)) { fine = false; break; }
             const uint32_t a = tc::smem_address(ring) + at * kSlice, bar = full + 8 * at;
             tc::barrier_expect(bar, kSlice);
-            tc::load_box(&p.w[0], a, bar, tile * 64, s * kDepth);
-            tc::load_box(&p.w[1], a + 8192, bar, tile * 64, s * kDepth);
-            tc::load_box(&p.x, a + kA, bar, s * kDepth, 0);
+            for (int i = 0; i < kFewCols / 64; ++i) tc::load_box(&p.w[0], a + i * 8192, bar, col + i * 64, k);
+            for (int i = 0; i < kFewCols / 64; ++i) tc::load_box(&p.w[1], a + kA + i * 8192, bar, col + i * 64, k);
+            tc::load_box(&p.x, a + 2 * kA, bar, k, 0);
         }
         if (!fine)
             for (unsigned i = issued > kR ? issued - kR : 0; i < issued; ++i) tc::barrier_wait(full + 8 * (i % kR), (i / kR) & 1, watch, true);
     } else if (warp == 1 && lane == 0) {
-        unsigned used = 0;
+        unsigned used = 0, count = 0;
+        bool fine = true;
         for (unsigned s = first; s < last; ++s, ++used) {
-            const unsigned at = used % kR;
-            if (!tc::barrier_wait(full + 8 * at, (used / kR) & 1, watch)) break;
+            const unsigned at = used % kR, acc = count & 1;
+            const bool begin = s == first || s % p.slices == 0;
+            if (begin && !tc::barrier_wait(taken + 8 * acc, ((count >> 1) & 1) ^ 1, watch)) { fine = false; break; }
+            if (!tc::barrier_wait(full + 8 * at, (used / kR) & 1, watch)) { fine = false; break; }
             tc::fence_after_sync();
-            const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA;
+            const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + 2 * kA, d = tmem + acc * kAcc;
 #pragma unroll
-            for (int k = 0; k < kDepth / 16; ++k)
-                tc::product(tmem, tc::tile_descriptor(a + k * 2048, true, 8192), tc::tile_descriptor(b + k * 32, false, 0), kInstruction, used || k);
+            for (int k = 0; k < kDepth / 16; ++k) {
+                const uint64_t x = tc::tile_descriptor(b + k * 32, false, 0);
+                tc::product(d, tc::tile_descriptor(a + k * 2048, true, 8192), x, kInstruction, !begin || k);
+                tc::product(d + kTokens, tc::tile_descriptor(a + kA + k * 2048, true, 8192), x, kInstruction, !begin || k);
+            }
             tc::commit(empty + 8 * at);
+            if (s + 1 == last || (s + 1) % p.slices == 0) {
+                tc::commit(ready + 8 * acc);
+                ++count;
+            }
         }
-        tc::commit(ready);
+        if (!fine) {
+            tc::commit(drained);
+            tc::barrier_wait(drained, 0, watch, true);
+        }
+    } else if (warp >= 4 && first < last) {
+        unsigned count = 0;
+        for (unsigned tile = first / p.slices; tile <= (last - 1) / p.slices; ++tile, ++count) {
+            const unsigned acc = count & 1;
+            const bool fine = tc::barrier_wait(ready + 8 * acc, (count >> 1) & 1, watch);
+            if (!__all_sync(0xffffffffu, fine)) break;
+            tc::fence_after_sync();
+            float* to = p.parts + (size_t)(tile + blockIdx.x) * p.tokens * 2 * kFewCols + (warp - 4) * 32 + lane;
+            for (unsigned t0 = 0; t0 < p.tokens; t0 += 16) {
+                float g[16], u[16];
+                tc::load_columns16(tmem + ((warp - 4) * 32 << 16) + acc * kAcc + t0, g);
+                tc::load_columns16(tmem + ((warp - 4) * 32 << 16) + acc * kAcc + kTokens + t0, u);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (t0 + i >= p.tokens) break;
+                    to[(t0 + i) * 2 * kFewCols] = g[i];
+                    to[(t0 + i) * 2 * kFewCols + kFewCols] = u[i];
+                }
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive(taken + 8 * acc);
+        }
     }
     __syncwarp();
-    // in every case the products issued are waited for: they read the ring, which is written next
-    tc::barrier_wait(ready, 0, watch, true);
-    tc::fence_after_sync();
-    __syncthreads();
-    const uint32_t sums = tc::smem_address(ring);   // [kTokens][128]
-#pragma unroll 1
-    for (int c = 0; c < kTokens; c += 16) {
-        float v[16];
-        tc::load_columns16(tmem + (warp * 32 << 16) + c, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) reinterpret_cast<float*>(ring)[(c + i) * 128 + threadIdx.x] = v[i];
-    }
     tc::fence_before_sync();
-    cluster_barrier();
+    __syncthreads();
     if (warp == 2) {
         tc::fence_after_sync();
-        tc::tmem_free(tmem, kTmem);
+        tc::tmem_free(tmem, 2 * kAcc);
     }
-    // this block's columns of the tile
-    const unsigned c0 = 64 * rank / parts, n_cols = 64 * (rank + 1) / parts - c0;
-    for (unsigned i = threadIdx.x; i < n_cols * p.tokens; i += 128) {
-        const unsigned c = c0 + i % n_cols, t = i / n_cols, f = tile * 64 + c;
-        float g = 0.0f, u = 0.0f;
-        for (unsigned r = 0; r < parts; ++r) {
-            g += cluster_load(sums + (t * 128 + c) * 4, r);
-            u += cluster_load(sums + (t * 128 + 64 + c) * 4, r);
-        }
-        if (f >= p.hidden) continue;
-        if (p.out[1]) {
-            static_cast<T*>(p.out[1])[t * p.ld[1] + f] = from_f32<T>(g);
-            static_cast<T*>(p.out[2])[t * p.ld[2] + f] = from_f32<T>(u);
-        }
-        static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(activate<false>(p.act, g, nullptr) * u);
+}
+
+// one block to 128 columns and a token
+template <class T>
+__global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_constant__ FewEnd p) {
+    const unsigned tile = blockIdx.x, t = blockIdx.y, f = tile * kFewCols + threadIdx.x, total = p.tiles * p.slices;
+    const unsigned b0 = run_of(tile * p.slices, p.blocks, total), b1 = run_of(tile * p.slices + p.slices - 1, p.blocks, total);
+    if (f >= p.hidden) return;
+    float g = 0.0f, u = 0.0f;
+    for (unsigned b = b0; b <= b1; ++b) {
+        const float* from = p.parts + ((size_t)(tile + b) * p.tokens + t) * 2 * kFewCols + threadIdx.x;
+        g += from[0];
+        u += from[kFewCols];
     }
-    cluster_barrier();   // the others may still read this block's sums
+    if (p.out[1]) {
+        static_cast<T*>(p.out[1])[t * p.ld[1] + f] = from_f32<T>(g);
+        static_cast<T*>(p.out[2])[t * p.ld[2] + f] = from_f32<T>(u);
+    }
+    static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(activate<false>(p.act, g, nullptr) * u);
 }
 
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
@@ -476,31 +507,22 @@ int glu_forward(const GluArgs& a, Operand x, Operand wg, Operand wu, ProductArgs
 }
 
 template <class T, int kTokens>
-int glu_few(const GluArgs& a, Operand x, Operand wg, Operand wu, int* flag, cudaStream_t s) {
+int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* flag, Scratch* scratch, cudaStream_t s) {
     FewArgs p = {};
     ZKB_TRY(tc::make_map(&p.x, kCode<T>, x.p, a.tokens, a.in, x.ld, kTokens));
     ZKB_TRY(tc::make_map(&p.w[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
     ZKB_TRY(tc::make_map(&p.w[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
-    p.tokens = (unsigned)a.tokens, p.hidden = (unsigned)a.hidden, p.slices = div_up(a.in, kDepth);
-    p.out[0] = a.h, p.out[1] = a.gate_out, p.out[2] = a.up_out;
-    p.ld[0] = a.ldh, p.ld[1] = a.ldg, p.ld[2] = a.ldu;
-    p.act = a.act, p.flag = flag;
-    // as many blocks to a tile as leave all of them resident at once
-    const unsigned tiles = div_up(a.hidden, 64), slots = kFewPerSm<kTokens> * sm_count();
-    p.blocks_per_tile = std::max(1u, std::min({8u, p.slices, slots / tiles}));
+    p.tokens = (unsigned)a.tokens, p.tiles = div_up(a.hidden, kFewCols), p.slices = div_up(a.in, kDepth), p.flag = flag;
+    const unsigned blocks = (unsigned)std::min((size_t)sm_count(), (size_t)p.tiles * p.slices);
+    p.parts = scratch->get_n<float>((size_t)(p.tiles + blocks) * p.tokens * 2 * kFewCols);
+    if (!p.parts) return ZKB_ERR_CUDA;
     const auto glu_few = glu_few_kernel<T, kTokens>;
     constexpr size_t smem = few_smem<kTokens>();
     ZKB_CUDA(cudaFuncSetAttribute(glu_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = p.blocks_per_tile, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(tiles * p.blocks_per_tile), c.blockDim = dim3(128), c.dynamicSmemBytes = smem, c.stream = s;
-    c.attrs = &cluster, c.numAttrs = 1;
-    if (g_profile_on) profile_begin("glu_few", s);
-    ZKB_CUDA(cudaLaunchKernelEx(&c, glu_few, p));
-    if (g_profile_on) profile_end(s);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    ZKB_LAUNCH(glu_few, blocks, kProductThreads, smem, s, p);
+    const FewEnd e = {p.parts, p.tokens, (unsigned)a.hidden, p.tiles, p.slices, blocks, {a.h, a.gate_out, a.up_out}, {a.ldh, a.ldg, a.ldu}, a.act};
+    const auto glu_few_finish = glu_few_finish_kernel<T>;
+    ZKB_LAUNCH(glu_few_finish, dim3(p.tiles, p.tokens), kFewCols, 0, s, e);
     return ZKB_OK;
 }
 
@@ -524,10 +546,10 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     p.act = a.act;
     p.flag = tc::wait_flag();
     if (!p.flag) return ZKB_ERR_CUDA;
-    if (a.tokens <= 16) return glu_few<T, 16>(a, x, wg, wu, p.flag, s);
-    if (a.tokens <= 32) return glu_few<T, 32>(a, x, wg, wu, p.flag, s);
-    if (a.tokens <= 64) return glu_few<T, 64>(a, x, wg, wu, p.flag, s);
-    if (a.tokens <= 128) return glu_few<T, 128>(a, x, wg, wu, p.flag, s);
+    if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, p.flag, &scratch, s);
+    if (a.tokens <= 32) return glu_few_launch<T, 32>(a, x, wg, wu, p.flag, &scratch, s);
+    if (a.tokens <= 64) return glu_few_launch<T, 64>(a, x, wg, wu, p.flag, &scratch, s);
+    if (a.tokens <= 128) return glu_few_launch<T, 128>(a, x, wg, wu, p.flag, &scratch, s);
     return glu_forward<T, 256>(a, x, wg, wu, p, s);
 }
 
