@@ -46,4 +46,25 @@ inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintpt
 // current device reaches, so that a host array or another device's tensor ends in an error and not in a fault.
 int check_device(const void* p, size_t align, const char* what);
 
+// A kernel that was launched beside its predecessor waits for that one's end and results; a kernel lets its successor be launched.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launch of a kernel that may start beside its predecessor on the stream: every thread of it that touches global memory, in
+// whichever way, does so after grid_wait().
+template <class... P, class... A>
+int launch_beside(const char* name, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchAttribute beside;
+    beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    beside.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = smem, c.stream = s, c.attrs = &beside;
+    c.numAttrs = g_profile_on ? 0 : 1;   // timed alone: the events around it would not order it
+    if (g_profile_on) profile_begin(name, s);
+    ZKB_CUDA(cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...));
+    if (g_profile_on) profile_end(s);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return ZKB_OK;
+}
+
 }  // namespace zkb

@@ -140,6 +140,8 @@ __global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __gr
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
+    grid_release();
+    grid_wait();
 
     const unsigned tiles = p.row_tiles * p.col_tiles, all = kForm == kPaired ? 2 * tiles : tiles;
     const unsigned slices = p.slices * kSums;
@@ -318,6 +320,8 @@ __global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_c
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
+    grid_release();
+    grid_wait();
 
     if (warp == 0 && lane == 0) {
         unsigned issued = 0;
@@ -392,10 +396,12 @@ __global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_c
     }
 }
 
-// one block to 128 columns and a token
+// One block to 128 columns and a token.  Its blocks are launched while glu_few_kernel still runs and wait for its end.
 template <class T>
 __global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_constant__ FewEnd p) {
     const unsigned tile = blockIdx.x, t = blockIdx.y, f = tile * kFewCols + threadIdx.x, total = p.tiles * p.slices;
+    grid_release();
+    grid_wait();
     const unsigned b0 = run_of(tile * p.slices, p.blocks, total), b1 = run_of(tile * p.slices + p.slices - 1, p.blocks, total);
     if (f >= p.hidden) return;
     float g = 0.0f, u = 0.0f;
@@ -417,6 +423,8 @@ __global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_c
 template <class T, int V>
 __global__ void __launch_bounds__(256) glu_split_kernel(const T* __restrict__ gate, size_t ldg, const T* __restrict__ up, size_t ldu, const T* __restrict__ dh,
                                                         size_t ldh, T* __restrict__ dg, T* __restrict__ du, size_t ld, size_t rows, size_t cols, int act) {
+    grid_release();
+    grid_wait();
     const size_t vecs = ld / 8;
     for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
         const size_t m = i / vecs, n = i % vecs * 8;
@@ -459,6 +467,8 @@ struct GluArgs {
 // whole 16 bytes: one pass over the operand before the products.
 template <class T>
 __global__ void __launch_bounds__(256) glu_align_kernel(const T* __restrict__ from, size_t ld_from, T* __restrict__ to, size_t ld_to, size_t rows, size_t cols) {
+    grid_release();
+    grid_wait();
     const size_t vecs = ld_to / 8;
     for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
         const size_t r = i / vecs, c = (i % vecs) * 8;
@@ -479,8 +489,8 @@ int align(Operand* x, size_t rows, size_t cols, Scratch* scratch, cudaStream_t s
     T* to = scratch->get_n<T>(rows * ld);
     if (!to) return ZKB_ERR_CUDA;
     const auto glu_align = glu_align_kernel<T>;
-    ZKB_LAUNCH(glu_align, (unsigned)std::min<size_t>((rows * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(x->p), x->ld, to, ld, rows,
-               cols);
+    ZKB_TRY(launch_beside("glu_align", glu_align, (unsigned)std::min<size_t>((rows * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(x->p), x->ld, to, ld, rows,
+               cols));
     *x = {to, ld};
     return ZKB_OK;
 }
@@ -491,8 +501,7 @@ int product_launch(const ProductArgs& p, cudaStream_t s) {
     constexpr size_t smem = product_smem<kCols>();
     ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const unsigned tiles = p.row_tiles * p.col_tiles * (kForm == kPaired ? 2 : 1);
-    ZKB_LAUNCH(glu_product, std::min(tiles, (kCols == 256 ? 1u : 2u) * sm_count()), kProductThreads, smem, s, p);
-    return ZKB_OK;
+    return launch_beside("glu_product", glu_product, std::min(tiles, (kCols == 256 ? 1u : 2u) * sm_count()), kProductThreads, smem, s, p);
 }
 
 template <class T> constexpr int kCode = std::is_same<T, __half>::value ? ZKB_F16 : ZKB_BF16;
@@ -519,11 +528,10 @@ int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* fla
     const auto glu_few = glu_few_kernel<T, kTokens>;
     constexpr size_t smem = few_smem<kTokens>();
     ZKB_CUDA(cudaFuncSetAttribute(glu_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    ZKB_LAUNCH(glu_few, blocks, kProductThreads, smem, s, p);
+    ZKB_TRY(launch_beside("glu_few", glu_few, blocks, kProductThreads, smem, s, p));
     const FewEnd e = {p.parts, p.tokens, (unsigned)a.hidden, p.tiles, p.slices, blocks, {a.h, a.gate_out, a.up_out}, {a.ldh, a.ldg, a.ldu}, a.act};
     const auto glu_few_finish = glu_few_finish_kernel<T>;
-    ZKB_LAUNCH(glu_few_finish, dim3(p.tiles, p.tokens), kFewCols, 0, s, e);
-    return ZKB_OK;
+    return launch_beside("glu_few_finish", glu_few_finish, dim3(p.tiles, p.tokens), kFewCols, 0, s, e);
 }
 
 template <class T>
@@ -568,8 +576,8 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     T* du = scratch.get_n<T>(a.tokens * ld);
     if (!dg || !du) return ZKB_ERR_CUDA;
     const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, 8> : glu_split_kernel<T, 1>;
-    ZKB_LAUNCH(glu_split, (unsigned)std::min<size_t>((a.tokens * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
-               static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld, a.tokens, F, a.act);
+    ZKB_TRY(launch_beside("glu_split", glu_split, (unsigned)std::min<size_t>((a.tokens * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
+               static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld, a.tokens, F, a.act));
     ProductArgs p = {};
     p.flag = tc::wait_flag();
     if (!p.flag) return ZKB_ERR_CUDA;

@@ -77,6 +77,12 @@ __device__ __forceinline__ void load_box(const CUtensorMap* m, uint32_t dst, uin
         : "memory");
 }
 
+// `bytes` consecutive bytes; both addresses and the size are multiples of 16
+__device__ __forceinline__ void load_bytes(uint32_t dst, unsigned long long src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // ---- tcgen05 -----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t at, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(cols) : "memory");
