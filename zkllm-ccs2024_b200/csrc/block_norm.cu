@@ -28,7 +28,7 @@ struct NormArgs {
     void *r, *z;
     size_t ldr, ldz;
     float *post_inv, *pre_inv;
-    float scale, eps;
+    float scale, eps, one_over_cols;
     int gate_kind;
     bool post_norm, pre_norm, gains_f32;
     unsigned slots, slot_bytes;
@@ -41,7 +41,7 @@ struct NormGradArgs {
     void *dx, *dy, *dgate;
     size_t lddx, lddy, lddgate;
     float* partial;        // [blocks][2][cols]: each block's sums over its rows
-    float scale, eps;
+    float scale, eps, one_over_cols;
     int gate_kind;
     bool post_norm, pre_norm, gains_f32, want_gate;
     unsigned slots, slot_bytes;
@@ -93,285 +93,495 @@ struct RowRing {
             }
     }
     __device__ __forceinline__ void wait(unsigned slot, uint32_t parity) const { tc::barrier_wait(bars + 8 * slot, parity, watch); }
-    __device__ __forceinline__ const T* row_of(int k, size_t row, unsigned slot) const {
-        const unsigned long long at = reinterpret_cast<unsigned long long>(src[k].p) + row * src[k].ld;
-        return reinterpret_cast<const T*>(slots + slot * slot_bytes + src[k].at + (at & 15));
+    __device__ __forceinline__ uint32_t row_of(int k, size_t row, unsigned slot) const {   // in shared memory
+        const unsigned at = (unsigned)reinterpret_cast<unsigned long long>(src[k].p) + (unsigned)row * (unsigned)src[k].ld;
+        return tc::smem_address(slots) + slot * slot_bytes + src[k].at + (at & 15);
     }
 };
 
-// Sums of K values over the threads of a row (blockDim.x of them, whole warps), for every thread.  `buf` holds 32 * K floats
-// of the row's own; a call may follow another on the same buffer only after a barrier.
-template <int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], float* buf) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    const unsigned warps = blockDim.x >> 5;
-    if (warps == 1) return;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int k = 0; k < K; ++k) buf[k * 32 + (threadIdx.x >> 5)] = v[k];
-    __syncthreads();
-    const unsigned lane = threadIdx.x & 31;
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = lane < warps ? buf[k * 32 + lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+// ---- pairs of 32-bit values: one instruction works on both ---------------------------------------------------------------------
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ Pair pair(float x) { return pair(x, x); }
+__device__ __forceinline__ void split(Pair p, float* lo, float* hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(p.v)); }
+__device__ __forceinline__ float total(Pair p) {
+    float lo, hi;
+    split(p, &lo, &hi);
+    return lo + hi;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair c;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
 }
 
-template <class T, int V>
-__device__ __forceinline__ void load_gain(const void* p, bool f32, size_t at, float (&out)[V]) {
+template <class T> __device__ __forceinline__ Pair widen(uint32_t two);
+template <> __device__ __forceinline__ Pair widen<bf16>(uint32_t two) { return pair(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)); }
+template <> __device__ __forceinline__ Pair widen<__half>(uint32_t two) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+    return pair(f.x, f.y);
+}
+template <class T> __device__ __forceinline__ uint32_t narrow(Pair p) {
+    float lo, hi;
+    split(p, &lo, &hi);
+    uint32_t two;
+    if constexpr (std::is_same<T, bf16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
+    return two;
+}
+
+// A thread's share of a row is kShare / G groups of G values (kShare: 8 or 16).  With alignment a group is the 16 bytes at (g * threads + thread) * G;
+// without, its values are `threads` apart, so that a warp's accesses still run together.  Places behind the row's end read as zero.
+template <class T, bool kAligned> constexpr int kGroup = kAligned ? kWide<T> : 4;
+
+template <bool kAligned, int G> struct Place {
+    unsigned at, step, cols;
+    __device__ __forceinline__ Place(int g, unsigned n) : at((g * blockDim.x * G) + (kAligned ? threadIdx.x * G : threadIdx.x)), step(blockDim.x), cols(n) {}
+    __device__ __forceinline__ bool any() const { return at < cols; }   // aligned: the whole group or nothing
+    __device__ __forceinline__ bool has(int j) const { return kAligned || at + j * step < cols; }
+    __device__ __forceinline__ unsigned of(int j) const { return kAligned ? at + j : at + j * step; }
+};
+// Where a row's values are read from: a slot of the ring, or global memory.
+template <class T> struct InSlot {
+    uint32_t p;
+    __device__ __forceinline__ uint4 wide(unsigned at) const {
+        uint4 x;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(p + at * (uint32_t)sizeof(T)));
+        return x;
+    }
+    __device__ __forceinline__ float one(unsigned at) const {
+        if constexpr (sizeof(T) == 4) {
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(p + at * 4));
+            return x;
+        } else {
+            unsigned short x;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(p + at * 2));
+            return to_f32<T>(*reinterpret_cast<const T*>(&x));
+        }
+    }
+};
+template <class T> struct InMemory {
+    const T* p;
+    __device__ __forceinline__ uint4 wide(unsigned at) const { return *reinterpret_cast<const uint4*>(p + at); }
+    __device__ __forceinline__ float one(unsigned at) const { return to_f32<T>(p[at]); }
+};
+template <class T, bool kAligned, int G, class From>
+__device__ __forceinline__ void load_group(const From& from, const Place<kAligned, G>& at, Pair (&out)[G / 2]) {
+    if constexpr (kAligned && sizeof(T) == 2) {
+        const uint4 x = from.wide(at.at);
+        out[0] = widen<T>(x.x), out[1] = widen<T>(x.y), out[2] = widen<T>(x.z), out[3] = widen<T>(x.w);
+    } else if constexpr (kAligned) {
+        const uint4 x = from.wide(at.at);
+        out[0] = pair(__uint_as_float(x.x), __uint_as_float(x.y)), out[1] = pair(__uint_as_float(x.z), __uint_as_float(x.w));
+    } else {
+#pragma unroll
+        for (int j = 0; j < G; j += 2) out[j / 2] = pair(at.has(j) ? from.one(at.of(j)) : 0.0f, at.has(j + 1) ? from.one(at.of(j + 1)) : 0.0f);
+    }
+}
+template <class T, bool kAligned, int G>
+__device__ __forceinline__ void store_group(T* p, const Place<kAligned, G>& at, const Pair (&in)[G / 2]) {
+    if constexpr (kAligned && sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p + at.at) = make_uint4(narrow<T>(in[0]), narrow<T>(in[1]), narrow<T>(in[2]), narrow<T>(in[3]));
+    } else {
+        float v[G];
+#pragma unroll
+        for (int j = 0; j < G; j += 2) split(in[j / 2], &v[j], &v[j + 1]);
+        if constexpr (kAligned) {
+            *reinterpret_cast<float4*>(p + at.at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+                if (at.has(j)) p[at.of(j)] = from_f32<T>(v[j]);
+        }
+    }
+}
+// a gain: of the tensors' type, in 32 bits, or ones
+template <class T, bool kAligned, int G>
+__device__ __forceinline__ void load_gain(const void* p, bool f32, const Place<kAligned, G>& at, Pair (&out)[G / 2]) {
     if (!p) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = 1.0f;
-    } else if (f32) {
-        constexpr int W = V < 4 ? V : 4;
+        for (int j = 0; j < G / 2; ++j) out[j] = pair(1.0f);
+    } else if (!f32) {
+        load_group<T, kAligned, G>(InMemory<T>{static_cast<const T*>(p)}, at, out);
+    } else if constexpr (kAligned) {
 #pragma unroll
-        for (int i = 0; i < V; i += W) {
-            float w[W];
-            load_vec<float, W>(static_cast<const float*>(p) + at + i, w);
-#pragma unroll
-            for (int j = 0; j < W; ++j) out[i + j] = w[j];
+        for (int j = 0; j < G; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at.at + j);
+            out[j / 2] = pair(x.x, x.y), out[j / 2 + 1] = pair(x.z, x.w);
         }
     } else {
-        load_vec<T, V>(static_cast<const T*>(p) + at, out);
+        load_group<float, kAligned, G>(InMemory<float>{static_cast<const float*>(p)}, at, out);
     }
 }
 
-// the gate's values at one place of a row; `values` is an ELEMENT gate's row, `row_gate` a ROW gate's value
-template <class T, int V>
-__device__ __forceinline__ void load_gate(const void* p, const T* values, int kind, bool gains_f32, float row_gate, size_t at, float (&out)[V]) {
-    if (kind == ZKB_GATE_ELEMENT) {
-        load_vec<T, V>(values + at, out);
-    } else if (kind == ZKB_GATE_CHANNEL) {
-        load_gain<T, V>(p, gains_f32, at, out);
-    } else {
+// Sums of up to 8 values over the block's threads (whole warps), for every thread.  Within a warp the values are dealt out while they are
+// added, so that eight take nine exchanges and not forty.  `buf`: 8 floats a warp; two calls on it need a barrier between.
+template <int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* buf) {
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    float mine;
+    if constexpr (K == 1) {
+        mine = v[0];
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = row_gate;
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (lane == 0) buf[warp] = mine;
+        __syncthreads();
+        mine = lane < warps ? buf[lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        v[0] = mine;
+    } else {
+        float w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = k < K ? v[k] : 0.0f;
+#pragma unroll
+        for (int o = 16, n = 4; n > 0; o >>= 1, n >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int k = 0; k < n; ++k) {
+                const float give = up ? w[k] : w[k + n];
+                w[k] = (up ? w[k + n] : w[k]) + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+        mine = w[0] + __shfl_xor_sync(0xffffffffu, w[0], 2);
+        mine += __shfl_xor_sync(0xffffffffu, mine, 1);          // value lane / 4 of this warp
+        if ((lane & 3) == 0) buf[warp * 8 + lane / 4] = mine;
+        __syncthreads();
+        mine = 0.0f;
+        for (unsigned i = lane / 8; i < warps; i += 4) mine += buf[i * 8 + lane % 8];
+        mine += __shfl_xor_sync(0xffffffffu, mine, 8);
+        mine += __shfl_xor_sync(0xffffffffu, mine, 16);
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, mine, k);
     }
 }
 
-// Bound by HBM: x and y are read once, r and z written once.  Each block takes rows blockIdx.x, blockIdx.x + gridDim.x, ...; with
-// kRing their values come through the ring, else straight from global memory (rows too long for two slots, or few rows, where
-// nothing could be fetched ahead).  NV vectors of V values to a thread.
-template <class T, int V, int NV, int kThreads, int kBlocks, bool kRing>
-__global__ void __launch_bounds__(kThreads, kBlocks) block_norm_kernel(const __grid_constant__ NormArgs a) {
+// How a kernel is laid out.  Slots: rows come through the ring and the values that all rows share (gains, a CHANNEL gate) stay in
+// registers: with the ring in shared memory little first-level cache is left, and read for each row they would come from L2, as many
+// bytes as the rows themselves.  Rows of more than 8192 values take 16 to a thread of 1024 and leave no registers for that, nor
+// is there room for their slots: they read straight from global memory.
+template <bool kAligned_, int kShare_, int kThreads_, int kBlocks_, bool kSlots_> struct Layout {
+    static constexpr bool kAligned = kAligned_, kSlots = kSlots_;
+    static constexpr int kShare = kShare_, kThreads = kThreads_, kBlocks = kBlocks_;
+};
+template <class T, class L> using From = std::conditional_t<L::kSlots, InSlot<T>, InMemory<T>>;
+template <class T, class L, int N>
+__device__ __forceinline__ From<T, L> row_from(const RowRing<T, N>& ring, const Source* src, int k, size_t row, unsigned slot) {
+    if constexpr (L::kSlots) return {ring.row_of(k, row, slot)};
+    else return {reinterpret_cast<const T*>(src[k].p + row * src[k].ld)};
+}
+
+// Bound by HBM: x and y are read once, r and z written once.  Each block takes rows blockIdx.x, blockIdx.x + gridDim.x, ...
+template <class T, class L>
+__global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int G = kGroup<T, L::kAligned>, NG = L::kShare / G;
+    typedef Place<L::kAligned, G> At;
     extern __shared__ __align__(16) char memory[];
-    __shared__ float sums[2 * 32];
+    __shared__ float sums[3 * 32];
     grid_release();
-    const RowRing<T, 3> ring(a.src, kRing ? a.cols : 0, kRing ? a.slots : 0, kRing ? a.slot_bytes : 0, memory, a.flag);
+    const RowRing<T, 3> ring(a.src, a.cols, a.slots, a.slot_bytes, memory, a.flag);
     grid_wait();
-    if (kRing && threadIdx.x == 0)
+    if (L::kSlots && threadIdx.x == 0)
         for (unsigned i = 0; i < a.slots && blockIdx.x + (size_t)i * gridDim.x < a.rows; ++i) ring.fetch(blockIdx.x + (size_t)i * gridDim.x, i);
     const bool branch = a.src[1].p != nullptr;
-    unsigned slot = 0;
+    const unsigned cols = (unsigned)a.cols;
+    // the gain after the branch times a CHANNEL gate, and the gain before the next
+    const auto load_e = [&](const At& at, Pair(&e)[G / 2]) {
+        load_gain<T>(a.post_gain, a.gains_f32, at, e);
+        if (a.gate_kind != ZKB_GATE_CHANNEL) return;
+        Pair g[G / 2];
+        load_gain<T>(a.gate, a.gains_f32, at, g);
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) e[j] = e[j] * g[j];
+    };
+    Pair held_e[L::kSlots ? NG : 1][G / 2], held_w[L::kSlots ? NG : 1][G / 2];
+    if constexpr (L::kSlots) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
+            if (!at.any()) continue;
+            load_e(at, held_e[g]);
+            load_gain<T>(a.pre_gain, a.gains_f32, at, held_w[g]);
+        }
+    }
+    unsigned slot = 0, odd = 0;
     uint32_t phase = 0;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        if (kRing) ring.wait(slot, phase);
-        const T* from[3];
+        if (L::kSlots) ring.wait(slot, phase);
+        Pair x[NG][G / 2], y[NG][G / 2], s2 = pair(0.0f);
+        float s[1];
+        const auto from_x = row_from<T, L>(ring, a.src, 0, row, slot), from_y = row_from<T, L>(ring, a.src, 1, row, slot),
+                   from_gate = row_from<T, L>(ring, a.src, 2, row, slot);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) from[k] = kRing ? ring.row_of(k, row, slot) : reinterpret_cast<const T*>(a.src[k].p + row * a.src[k].ld);
-        float x[NV][V], y[NV][V];
-        float s[1] = {0.0f};
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i][j] = y[i][j] = 0.0f;
-            if (at >= a.cols) continue;
-            load_vec<T, V>(from[0] + at, x[i]);
+            for (int j = 0; j < G / 2; ++j) x[g][j] = y[g][j] = pair(0.0f);
+            if (!at.any()) continue;
+            load_group<T>(from_x, at, x[g]);
             if (!branch) continue;
-            load_vec<T, V>(from[1] + at, y[i]);
+            load_group<T>(from_y, at, y[g]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += y[i][j] * y[i][j];
+            for (int j = 0; j < G / 2; ++j) s2 = fma(y[g][j], y[g][j], s2);
         }
         float post_inv = 1.0f;
         if (a.post_norm) {
-            row_sum<1>(s, sums);
-            post_inv = rsqrtf(s[0] / (float)a.cols + a.eps);
+            s[0] = total(s2);
+            row_sums<1>(s, sums);
+            post_inv = rsqrtf(s[0] * a.one_over_cols + a.eps);
             if (threadIdx.x == 0 && a.post_inv) a.post_inv[row] = post_inv;
         }
-        if (branch) {
-            const float row_gate = a.gate_kind == ZKB_GATE_ROW ? to_f32<T>(static_cast<const T*>(a.gate)[row]) : 1.0f;
+        s2 = pair(0.0f);
+        T* const r_row = static_cast<T*>(a.r) + row * a.ldr;
+        const Pair by = pair(a.scale * post_inv * (a.gate_kind == ZKB_GATE_ROW ? to_f32<T>(static_cast<const T*>(a.gate)[row]) : 1.0f));
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-                if (at >= a.cols) continue;
-                float w[V], g[V];
-                load_gain<T, V>(a.post_gain, a.gains_f32, at, w);
-                load_gate<T, V>(a.gate, from[2], a.gate_kind, a.gains_f32, row_gate, at, g);
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
+            if (!at.any()) continue;
+            if (branch) {
+                Pair w[G / 2];
+                if constexpr (!L::kSlots) load_e(at, w);
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[i][j] += a.scale * g[j] * (y[i][j] * post_inv * w[j]);
+                for (int j = 0; j < G / 2; ++j) y[g][j] = y[g][j] * (L::kSlots ? held_e[L::kSlots ? g : 0][j] : w[j]);
+                if (a.gate_kind == ZKB_GATE_ELEMENT) {
+                    load_group<T>(from_gate, at, w);
+#pragma unroll
+                    for (int j = 0; j < G / 2; ++j) y[g][j] = y[g][j] * w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < G / 2; ++j) x[g][j] = fma(y[g][j], by, x[g][j]);
             }
-        }
-        s[0] = 0.0f;
+            if (a.r) store_group<T>(r_row, at, x[g]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-            if (a.r && at < a.cols) store_vec<T, V>(static_cast<T*>(a.r) + row * a.ldr + at, x[i]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += x[i][j] * x[i][j];
+            for (int j = 0; j < G / 2; ++j) s2 = fma(x[g][j], x[g][j], s2);
         }
-        row_sum<1>(s, sums + 32);
-        __syncthreads();      // one warp alone passes no barrier in row_sum; every thread is done with this row's slot
-        if (kRing) {
+        s[0] = total(s2);
+        row_sums<1>(s, sums + 32 + 32 * odd);      // behind its barrier every thread has read this row's slot
+        odd ^= 1;
+        if (L::kSlots) {
             const size_t next = row + (size_t)a.slots * gridDim.x;
             if (threadIdx.x == 0 && next < a.rows) ring.fetch(next, slot);
             if (++slot == a.slots) { slot = 0; phase ^= 1; }
         }
         if (!a.pre_norm) continue;
-        const float inv = rsqrtf(s[0] / (float)a.cols + a.eps);
+        const float inv = rsqrtf(s[0] * a.one_over_cols + a.eps);
         if (threadIdx.x == 0 && a.pre_inv) a.pre_inv[row] = inv;
         if (!a.z) continue;
+        T* const z_row = static_cast<T*>(a.z) + row * a.ldz;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-            if (at >= a.cols) continue;
-            float w[V];
-            load_gain<T, V>(a.pre_gain, a.gains_f32, at, w);
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
+            if (!at.any()) continue;
+            Pair w[G / 2];
+            if constexpr (!L::kSlots) load_gain<T>(a.pre_gain, a.gains_f32, at, w);
 #pragma unroll
-            for (int j = 0; j < V; ++j) w[j] *= x[i][j] * inv;
-            store_vec<T, V>(static_cast<T*>(a.z) + row * a.ldz + at, w);
+            for (int j = 0; j < G / 2; ++j) w[j] = (L::kSlots ? held_w[L::kSlots ? g : 0][j] : w[j]) * (x[g][j] * pair(inv));
+            store_group<T>(z_row, at, w);
         }
     }
 }
 
-// The gradients.  With p = dz * w_pre, the gradient of r is d = dr + inv (p - r inv^2 mean(p r)); that of the branch before
-// its norm follows from a * gate * d * w_post in the same way.  Two sums over rows serve all three vectors: dz r inv gives the
-// gain before the next branch, and S = d yn (times the gate where that is not the same for all rows) both the other gain,
-// a gate S, and a CHANNEL gate, a w_post S.  Each block keeps its rows' share of them in registers; norm_reduce_kernel adds the
-// shares in the order of the blocks, so that a result does not depend on timing.
-template <class T, int V, int NV, int kThreads, int kBlocks, bool kRing>
-__global__ void __launch_bounds__(kThreads, kBlocks) block_norm_backward_kernel(const __grid_constant__ NormGradArgs a) {
+// The gradients.  With p = dz w_pre, the gradient of r is d = dr + inv (p - r b), b = inv^2 mean(p r); with e = gate w_post, that of y
+// is a ip (e d - y ip^2 mean(e d y)).  The last mean needs no pass of its own: by the first formula sum(e d y) =
+// sum(e y dr) + inv sum(e y p) - inv b sum(e y r), so that one round of six sums serves both norms.
+//
+// Two sums over rows serve all three vectors: dz r inv gives the gain before the next branch, and S = d y ip (times the gate where
+// that differs from row to row) both the other gain, a gate S, and a CHANNEL gate, a w_post S.  Each block keeps its rows'
+// share of them in registers; norm_reduce_kernel adds the shares in the order of the blocks, so that a result does not depend on timing.
+template <class T, class L>
+__global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_backward_kernel(const __grid_constant__ NormGradArgs a) {
+    constexpr int G = kGroup<T, L::kAligned>, NG = L::kShare / G;
+    typedef Place<L::kAligned, G> At;
     extern __shared__ __align__(16) char memory[];
-    __shared__ float sums[5 * 32];
+    __shared__ float sums[2][8 * 32];
     grid_release();
-    const RowRing<T, 5> ring(a.src, kRing ? a.cols : 0, kRing ? a.slots : 0, kRing ? a.slot_bytes : 0, memory, a.flag);
+    const RowRing<T, 5> ring(a.src, a.cols, a.slots, a.slot_bytes, memory, a.flag);
     grid_wait();
-    if (kRing && threadIdx.x == 0)
+    if (L::kSlots && threadIdx.x == 0)
         for (unsigned i = 0; i < a.slots && blockIdx.x + (size_t)i * gridDim.x < a.rows; ++i) ring.fetch(blockIdx.x + (size_t)i * gridDim.x, i);
-    const bool branch = a.src[2].p != nullptr, more = a.src[3].p != nullptr;
-    const float count = (float)a.cols;
-    float acc_pre[NV][V], acc_post[NV][V];
+    const bool branch = a.src[2].p != nullptr, more = a.src[3].p != nullptr, element = a.gate_kind == ZKB_GATE_ELEMENT;
+    const unsigned cols = (unsigned)a.cols;
+    // the gain after the branch times a CHANNEL gate
+    const auto load_e = [&](const At& at, Pair(&e)[G / 2]) {
+        load_gain<T>(a.post_gain, a.gains_f32, at, e);
+        if (a.gate_kind != ZKB_GATE_CHANNEL) return;
+        Pair g[G / 2];
+        load_gain<T>(a.gate, a.gains_f32, at, g);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < G / 2; ++j) e[j] = e[j] * g[j];
+    };
+    Pair acc_pre[NG][G / 2], acc_post[NG][G / 2], held_e[L::kSlots ? NG : 1][G / 2], held_w[L::kSlots ? NG : 1][G / 2];
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc_pre[i][j] = acc_post[i][j] = 0.0f;
-    unsigned slot = 0;
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) acc_pre[g][j] = acc_post[g][j] = pair(0.0f);
+        const At at(g, cols);
+        if (!L::kSlots || !at.any()) continue;
+        load_e(at, held_e[L::kSlots ? g : 0]);
+        load_gain<T>(a.pre_gain, a.gains_f32, at, held_w[L::kSlots ? g : 0]);
+    }
+    const auto pre_gain = [&](int g, const At& at, Pair(&w)[G / 2]) {
+        if constexpr (!L::kSlots) load_gain<T>(a.pre_gain, a.gains_f32, at, w);
+        else
+#pragma unroll
+            for (int j = 0; j < G / 2; ++j) w[j] = held_w[g][j];
+    };
+    const auto post_gain = [&](int g, const At& at, Pair(&w)[G / 2]) {
+        if constexpr (!L::kSlots) load_e(at, w);
+        else
+#pragma unroll
+            for (int j = 0; j < G / 2; ++j) w[j] = held_e[g][j];
+    };
+    unsigned slot = 0, odd = 0, done = 0;   // done: the slot of the row before
     uint32_t phase = 0;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        if (kRing) ring.wait(slot, phase);
-        const T* from[5];
+        if (L::kSlots) ring.wait(slot, phase);
+        const auto from_r = row_from<T, L>(ring, a.src, 0, row, slot), from_dz = row_from<T, L>(ring, a.src, 1, row, slot),
+                   from_y = row_from<T, L>(ring, a.src, 2, row, slot), from_dr = row_from<T, L>(ring, a.src, 3, row, slot),
+                   from_gate = row_from<T, L>(ring, a.src, 4, row, slot);
+        Pair rr = pair(0.0f), pr = rr, yy = rr, eyd = rr, eyp = rr, eyr = rr;
 #pragma unroll
-        for (int k = 0; k < 5; ++k) from[k] = kRing ? ring.row_of(k, row, slot) : reinterpret_cast<const T*>(a.src[k].p + row * a.src[k].ld);
-        float s[3] = {0.0f, 0.0f, 0.0f};   // r^2, p r, y^2
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-            if (at >= a.cols) continue;
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
+            if (!at.any()) continue;
+            Pair r[G / 2], p[G / 2], w[G / 2];
             if (a.pre_norm) {
-                float r[V], dz[V], w[V];
-                load_vec<T, V>(from[0] + at, r);
-                load_vec<T, V>(from[1] + at, dz);
-                load_gain<T, V>(a.pre_gain, a.gains_f32, at, w);
+                load_group<T>(from_r, at, r);
+                load_group<T>(from_dz, at, p);
+                pre_gain(g, at, w);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    s[0] += r[j] * r[j];
-                    s[1] += dz[j] * w[j] * r[j];
+                for (int j = 0; j < G / 2; ++j) {
+                    p[j] = p[j] * w[j];
+                    rr = fma(r[j], r[j], rr);
+                    pr = fma(p[j], r[j], pr);
                 }
             }
-            if (a.post_norm) {
-                float y[V];
-                load_vec<T, V>(from[2] + at, y);
+            if (branch) {
+                Pair y[G / 2];
+                load_group<T>(from_y, at, y);
+                post_gain(g, at, w);
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[2] += y[j] * y[j];
+                for (int j = 0; j < G / 2; ++j) {
+                    yy = fma(y[j], y[j], yy);
+                    y[j] = y[j] * w[j];
+                }
+                if (element) {
+                    load_group<T>(from_gate, at, w);
+#pragma unroll
+                    for (int j = 0; j < G / 2; ++j) y[j] = y[j] * w[j];
+                }
+                if (a.pre_norm)
+#pragma unroll
+                    for (int j = 0; j < G / 2; ++j) {
+                        eyp = fma(y[j], p[j], eyp);
+                        eyr = fma(y[j], r[j], eyr);
+                    }
+                if (more) {
+                    load_group<T>(from_dr, at, w);
+#pragma unroll
+                    for (int j = 0; j < G / 2; ++j) eyd = fma(y[j], w[j], eyd);
+                }
             }
         }
-        row_sum<3>(s, sums);
-        const float inv = a.pre_norm ? rsqrtf(s[0] / count + a.eps) : 0.0f;
-        const float back = inv * inv * s[1] / count;
-        const float post_inv = a.post_norm ? rsqrtf(s[2] / count + a.eps) : 1.0f;
+        float s[6] = {total(rr), total(pr), total(yy), total(eyd), total(eyp), total(eyr)};
+        row_sums<6>(s, sums[odd]);
+        odd ^= 1;
+        if (L::kSlots) {   // behind the barrier in row_sums every thread is done with the row before
+            if (threadIdx.x == 0 && row >= gridDim.x && a.slots > 1) {
+                const size_t next = row + (size_t)(a.slots - 1) * gridDim.x;
+                if (next < a.rows) ring.fetch(next, done);
+            }
+            done = slot;
+            if (++slot == a.slots) { slot = 0; phase ^= 1; }
+        }
+        const float inv = a.pre_norm ? rsqrtf(s[0] * a.one_over_cols + a.eps) : 0.0f, b = inv * inv * s[1] * a.one_over_cols;
+        const float post_inv = a.post_norm ? rsqrtf(s[2] * a.one_over_cols + a.eps) : 1.0f;
+        const float edy = s[3] + inv * (s[4] - b * s[5]);
+        // a ROW gate is not in e: it scales the whole branch
         const float row_gate = a.gate_kind == ZKB_GATE_ROW ? to_f32<T>(static_cast<const T*>(a.gate)[row]) : 1.0f;
-        const bool by_row = a.gate_kind == ZKB_GATE_ROW || a.gate_kind == ZKB_GATE_ELEMENT;
-        float q[2] = {0.0f, 0.0f};          // gate w_post d y, w_post d y
-        float d[NV][V];
+        if (a.want_gate && a.gate_kind == ZKB_GATE_ROW && threadIdx.x == 0) static_cast<T*>(a.dgate)[row] = from_f32<T>(a.scale * post_inv * edy);
+        const float by = a.scale * row_gate * post_inv;
+        const Pair by2 = pair(by), less = pair(a.post_norm ? -by * post_inv * post_inv * edy * a.one_over_cols : 0.0f), inv2 = pair(inv), b2 = pair(-b);
+        const Pair share = pair(post_inv * row_gate), dg_by = pair(a.scale * post_inv);
+        T* const dx_row = static_cast<T*>(a.dx) + row * a.lddx;
+        T* const dy_row = static_cast<T*>(a.dy) + row * a.lddy;
+        T* const dgate_row = static_cast<T*>(a.dgate) + row * a.lddgate;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-            if (at >= a.cols) continue;
+        for (int g = 0; g < NG; ++g) {
+            const At at(g, cols);
+            if (!at.any()) continue;
+            Pair d[G / 2], w[G / 2];
 #pragma unroll
-            for (int j = 0; j < V; ++j) d[i][j] = 0.0f;
-            if (more) load_vec<T, V>(from[3] + at, d[i]);
+            for (int j = 0; j < G / 2; ++j) d[j] = pair(0.0f);
+            if (more) load_group<T>(from_dr, at, d);
             if (a.pre_norm) {
-                float r[V], dz[V], w[V];
-                load_vec<T, V>(from[0] + at, r);
-                load_vec<T, V>(from[1] + at, dz);
-                load_gain<T, V>(a.pre_gain, a.gains_f32, at, w);
+                Pair r[G / 2], dz[G / 2];
+                load_group<T>(from_r, at, r);
+                load_group<T>(from_dz, at, dz);
+                pre_gain(g, at, w);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    acc_pre[i][j] += dz[j] * (r[j] * inv);
-                    d[i][j] += inv * (dz[j] * w[j] - r[j] * back);
+                for (int j = 0; j < G / 2; ++j) {
+                    acc_pre[g][j] = fma(dz[j] * r[j], inv2, acc_pre[g][j]);
+                    d[j] = fma(fma(r[j], b2, dz[j] * w[j]), inv2, d[j]);
                 }
             }
-            if (a.dx) store_vec<T, V>(static_cast<T*>(a.dx) + row * a.lddx + at, d[i]);
+            if (a.dx) store_group<T>(dx_row, at, d);
             if (!branch) continue;
-            float y[V], wp[V], g[V];
-            load_vec<T, V>(from[2] + at, y);
-            load_gain<T, V>(a.post_gain, a.gains_f32, at, wp);
-            load_gate<T, V>(a.gate, from[4], a.gate_kind, a.gains_f32, row_gate, at, g);
-            if (a.gate_kind == ZKB_GATE_ELEMENT && a.want_gate) {
-                float dg[V];
+            Pair y[G / 2];
+            load_group<T>(from_y, at, y);
+            post_gain(g, at, w);
+            if (element) {
+                Pair gate[G / 2], dy[G / 2];
+                load_group<T>(from_gate, at, gate);
 #pragma unroll
-                for (int j = 0; j < V; ++j) dg[j] = a.scale * d[i][j] * (y[j] * post_inv * wp[j]);
-                store_vec<T, V>(static_cast<T*>(a.dgate) + row * a.lddgate + at, dg);
-            }
+                for (int j = 0; j < G / 2; ++j) {
+                    dy[j] = d[j] * y[j];
+                    acc_post[g][j] = fma(dy[j] * gate[j], share, acc_post[g][j]);
+                    dy[j] = dy[j] * (w[j] * dg_by);
+                    w[j] = w[j] * gate[j];
+                }
+                if (a.want_gate) store_group<T>(dgate_row, at, dy);
+            } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float dy = d[i][j] * y[j];
-                acc_post[i][j] += by_row ? g[j] * (dy * post_inv) : dy * post_inv;
-                q[0] += g[j] * wp[j] * dy;
-                q[1] += wp[j] * dy;
-                d[i][j] *= g[j] * wp[j];    // from here on: the gradient of the normed branch times its gain, less the scale
+                for (int j = 0; j < G / 2; ++j) acc_post[g][j] = fma(d[j] * y[j], share, acc_post[g][j]);
             }
-        }
-        row_sum<2>(q, sums + 96);
-        if (branch) {
-            if (a.want_gate && a.gate_kind == ZKB_GATE_ROW && threadIdx.x == 0)
-                static_cast<T*>(a.dgate)[row] = from_f32<T>(a.scale * post_inv * q[1]);
-            const float post_back = a.post_norm ? post_inv * post_inv * q[0] / count : 0.0f;
             if (a.dy) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-                    if (at >= a.cols) continue;
-                    float y[V];
-                    load_vec<T, V>(from[2] + at, y);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) y[j] = a.scale * post_inv * (d[i][j] - y[j] * post_back);
-                    store_vec<T, V>(static_cast<T*>(a.dy) + row * a.lddy + at, y);
-                }
+                for (int j = 0; j < G / 2; ++j) d[j] = fma(d[j] * w[j], by2, y[j] * less);
+                store_group<T>(dy_row, at, d);
             }
         }
-        __syncthreads();      // every thread is done with this row's slot and sums
-        if (kRing) {
-            const size_t next = row + (size_t)a.slots * gridDim.x;
-            if (threadIdx.x == 0 && next < a.rows) ring.fetch(next, slot);
-            if (++slot == a.slots) { slot = 0; phase ^= 1; }
+        if (L::kSlots && a.slots == 1) {
+            __syncthreads();
+            if (threadIdx.x == 0 && row + gridDim.x < a.rows) ring.fetch(row + gridDim.x, 0);
         }
     }
     if (!a.partial) return;
     float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const size_t at = ((size_t)i * blockDim.x + threadIdx.x) * V;
-        if (at >= a.cols) continue;
+    for (int g = 0; g < NG; ++g) {
+        const At at(g, cols);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            out[at + j] = acc_pre[i][j];
-            out[a.cols + at + j] = acc_post[i][j];
+        for (int j = 0; j < G / 2; ++j) {
+            float v[2], u[2];
+            split(acc_pre[g][j], &v[0], &v[1]);
+            split(acc_post[g][j], &u[0], &u[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (at.any() && at.has(2 * j + k)) {
+                    out[at.of(2 * j + k)] = v[k];
+                    out[a.cols + at.of(2 * j + k)] = u[k];
+                }
         }
     }
 }
@@ -408,11 +618,9 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const __grid_constant_
     if (blockIdx.y == 0) {
         put(a.dpre, s);
     } else {
-        float g[1], w[1];
-        load_gain<T, 1>(a.gate, a.gains_f32, c, g);
-        load_gain<T, 1>(a.post_gain, a.gains_f32, c, w);
-        put(a.dpost, a.scale * g[0] * s);
-        put(a.dgate, a.scale * w[0] * s);
+        const auto one = [&](const void* p) { return !p ? 1.0f : a.gains_f32 ? static_cast<const float*>(p)[c] : to_f32<T>(static_cast<const T*>(p)[c]); };
+        put(a.dpost, a.scale * one(a.gate) * s);
+        put(a.dgate, a.scale * one(a.post_gain) * s);
     }
 }
 
@@ -420,68 +628,55 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const __grid_constant_
 unsigned row_threads(size_t cols, unsigned per) { return std::max(32u, div_up(div_up(cols, per), 32) * 32); }
 
 constexpr size_t kRingHead = 16 * 8;
-// The grid of a kernel over rows, and its ring: as many blocks as are resident, each with as many slots as fit.  Without a second
-// row to a block, or room for two slots, there is no ring (slots = 0).
-template <class Kernel>
-int plan_rows(Kernel ringed, Kernel direct, unsigned threads, Source* src, int matrices, size_t rows, size_t row_bytes, Kernel* kernel, unsigned* blocks,
-              unsigned* slots, unsigned* slot_bytes, size_t* smem) {
+// The grid of a kernel over rows, and its ring: as many blocks as are resident, each with as many slots as fit.
+template <class L, class Kernel, class Args>
+int plan_rows(Kernel kernel, unsigned threads, int matrices, size_t es, Args* a, unsigned* blocks, size_t* smem) {
     int resident = 0;
-    ZKB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, ringed, threads, 0));
+    ZKB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, kRingHead));
     resident = std::max(1, resident);
-    size_t slot = 0;
-    for (int k = 0; k < matrices; ++k) {
-        src[k].at = (unsigned)slot;
-        if (src[k].p) slot += row_bytes;
-    }
-    *slot_bytes = (unsigned)slot;
-    slot = std::max<size_t>(slot, 16);
-    const size_t room = 220 * 1024;
-    while (resident > 1 && (room / resident - 2048 - kRingHead) / slot < 2) --resident;   // 1 KB of each block's share is the system's
-    const size_t fit = std::min<size_t>(8, (room / resident - 2048 - kRingHead) / slot);
-    if (fit >= 2 && rows > (size_t)resident * sm_count()) {
-        *kernel = ringed;
-        *slots = (unsigned)fit;
-        *smem = kRingHead + fit * slot;
-        *blocks = (unsigned)resident * sm_count();
-        ZKB_CUDA(cudaFuncSetAttribute(ringed, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)*smem));
-        return ZKB_OK;
-    }
-    ZKB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, direct, threads, kRingHead));
-    *kernel = direct;
-    *slots = 0;
     *smem = kRingHead;
-    *blocks = (unsigned)std::min<size_t>(rows, (size_t)std::max(1, resident) * sm_count());
+    if (L::kSlots) {
+        size_t slot = 0;
+        for (int k = 0; k < matrices; ++k) {
+            a->src[k].at = (unsigned)slot;
+            if (a->src[k].p) slot += slot_row_bytes(a->cols, es);
+        }
+        a->slot_bytes = (unsigned)slot;
+        slot = std::max<size_t>(slot, 16);
+        const size_t room = 224 * 1024, other = 4096 + kRingHead;   // of each block's share, 1 KB is the system's and up to 3 KB the sums'
+        const auto fit = [&](int blocks_per_sm) { return (room / blocks_per_sm - other) / slot; };
+        while (resident > 1 && fit(resident) < 3) --resident;
+        a->slots = (unsigned)std::min<size_t>(8, std::max<size_t>(1, fit(resident)));
+        *smem += a->slots * slot;
+        ZKB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)*smem));
+    }
+    *blocks = (unsigned)std::min<size_t>(a->rows, (size_t)resident * sm_count());
     return ZKB_OK;
 }
 
-template <class T, int V, int NV>
+template <class T, class L>
 int norm_launch(NormArgs a, cudaStream_t s) {
-    const unsigned threads = row_threads(a.cols, V * NV);
-    const auto pick = [&](bool ring) {
-        return threads > 512 ? (ring ? block_norm_kernel<T, V, NV, 1024, 1, true> : block_norm_kernel<T, V, NV, 1024, 1, false>)
-                             : (ring ? block_norm_kernel<T, V, NV, 512, 2, true> : block_norm_kernel<T, V, NV, 512, 2, false>);
-    };
-    auto kernel = pick(true);
+    const unsigned threads = row_threads(a.cols, L::kShare);
+    const auto kernel = block_norm_kernel<T, L>;
     unsigned blocks;
     size_t smem;
-    ZKB_TRY(plan_rows(pick(true), pick(false), threads, a.src, 3, a.rows, slot_row_bytes(a.cols, sizeof(T)), &kernel, &blocks, &a.slots,
-                      &a.slot_bytes, &smem));
+    ZKB_TRY((plan_rows<L>(kernel, threads, 3, sizeof(T), &a, &blocks, &smem)));
     return launch_beside("block_norm", kernel, blocks, threads, smem, s, a);
 }
+template <class T, bool kAligned>
+int norm_launch(const NormArgs& a, cudaStream_t s) {
+    if (a.cols <= 4096) return norm_launch<T, Layout<kAligned, 8, 512, 2, true>>(a, s);
+    if (a.cols <= 8192) return norm_launch<T, Layout<kAligned, 8, 1024, 1, true>>(a, s);
+    return norm_launch<T, Layout<kAligned, 16, 1024, 1, false>>(a, s);
+}
 
-template <class T, int V, int NV>
+template <class T, class L>
 int norm_backward_launch(NormGradArgs a, void* dpost, void* dpre, cudaStream_t s) {
-    const unsigned threads = row_threads(a.cols, V * NV);
-    const auto pick = [&](bool ring) {
-        return threads > 512 ? (ring ? block_norm_backward_kernel<T, V, NV, 1024, 1, true> : block_norm_backward_kernel<T, V, NV, 1024, 1, false>)
-               : threads > 320 ? (ring ? block_norm_backward_kernel<T, V, NV, 512, 1, true> : block_norm_backward_kernel<T, V, NV, 512, 1, false>)
-                               : (ring ? block_norm_backward_kernel<T, V, NV, 320, 2, true> : block_norm_backward_kernel<T, V, NV, 320, 2, false>);
-    };
-    auto kernel = pick(true);
+    const unsigned threads = row_threads(a.cols, L::kShare);
+    const auto kernel = block_norm_backward_kernel<T, L>;
     unsigned blocks;
     size_t smem;
-    ZKB_TRY(plan_rows(pick(true), pick(false), threads, a.src, 5, a.rows, slot_row_bytes(a.cols, sizeof(T)), &kernel, &blocks, &a.slots,
-                      &a.slot_bytes, &smem));
+    ZKB_TRY((plan_rows<L>(kernel, threads, 5, sizeof(T), &a, &blocks, &smem)));
     Scratch scratch(s);
     const bool channel = a.want_gate && a.gate_kind == ZKB_GATE_CHANNEL;
     if (dpre || dpost || channel) {
@@ -494,15 +689,12 @@ int norm_backward_launch(NormGradArgs a, void* dpost, void* dpre, cudaStream_t s
                               a.post_gain, a.scale, a.gains_f32};
     return launch_beside("norm_reduce", norm_reduce_kernel<T>, dim3(div_up(a.cols, 32), 2), 256, 0, s, n);
 }
-
-// 16 values to a thread: more would not leave two blocks their registers, fewer would make the sums over a row cost more than the row
-template <class T>
-int norm_dispatch(const NormArgs& a, bool wide, cudaStream_t s) {
-    return wide ? norm_launch<T, kWide<T>, 16 / kWide<T>>(a, s) : norm_launch<T, 1, 16>(a, s);
-}
-template <class T>
-int norm_backward_dispatch(const NormGradArgs& a, bool wide, void* dpost, void* dpre, cudaStream_t s) {
-    return wide ? norm_backward_launch<T, kWide<T>, 16 / kWide<T>>(a, dpost, dpre, s) : norm_backward_launch<T, 1, 16>(a, dpost, dpre, s);
+template <class T, bool kAligned>
+int norm_backward_launch(const NormGradArgs& a, void* dpost, void* dpre, cudaStream_t s) {
+    if (a.cols <= 2560) return norm_backward_launch<T, Layout<kAligned, 8, 320, 2, true>>(a, dpost, dpre, s);
+    if (a.cols <= 5120) return norm_backward_launch<T, Layout<kAligned, 8, 640, 1, true>>(a, dpost, dpre, s);
+    if (a.cols <= 8192) return norm_backward_launch<T, Layout<kAligned, 16, 512, 1, true>>(a, dpost, dpre, s);
+    return norm_backward_launch<T, Layout<kAligned, 16, 1024, 1, false>>(a, dpost, dpre, s);
 }
 
 // what both directions check
@@ -575,13 +767,13 @@ int zkb_block_norm(int dtype, int gains_dtype, size_t rows, size_t cols, const v
     a.src[2] = {gate_kind == ZKB_GATE_ELEMENT ? static_cast<const char*>(d_gate) : nullptr, gate_ld * es};
     a.gate = d_gate, a.post_gain = d_post_gain, a.pre_gain = d_pre_gain;
     a.r = d_r, a.z = d_z, a.ldr = ldr, a.ldz = ldz, a.post_inv = d_post_inv, a.pre_inv = d_pre_inv;
-    a.scale = residual_scale, a.eps = eps, a.gate_kind = gate_kind;
+    a.scale = residual_scale, a.eps = eps, a.one_over_cols = (float)(1.0 / (double)cols), a.gate_kind = gate_kind;
     a.post_norm = post_norm != 0, a.pre_norm = pre_norm != 0, a.gains_f32 = gains_dtype == ZKB_F32;
     if (!(a.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
     const cudaStream_t s = as_stream(stream);
-    if (dtype == ZKB_F32) return norm_dispatch<float>(a, wide, s);
-    if (dtype == ZKB_F16) return norm_dispatch<__half>(a, wide, s);
-    return norm_dispatch<bf16>(a, wide, s);
+    if (dtype == ZKB_F32) return wide ? norm_launch<float, true>(a, s) : norm_launch<float, false>(a, s);
+    if (dtype == ZKB_F16) return wide ? norm_launch<__half, true>(a, s) : norm_launch<__half, false>(a, s);
+    return wide ? norm_launch<bf16, true>(a, s) : norm_launch<bf16, false>(a, s);
 }
 
 int zkb_block_norm_backward(int dtype, int gains_dtype, size_t rows, size_t cols, const void* d_r, size_t ldr, const void* d_y, size_t ldy, int post_norm,
@@ -636,12 +828,12 @@ int zkb_block_norm_backward(int dtype, int gains_dtype, size_t rows, size_t cols
     a.src[4] = {element ? static_cast<const char*>(d_gate) : nullptr, gate_ld * es};
     a.gate = d_gate, a.post_gain = d_post_gain, a.pre_gain = d_pre_gain;
     a.dx = d_dx, a.dy = d_dy, a.dgate = d_dgate, a.lddx = lddx, a.lddy = lddy, a.lddgate = lddgate;
-    a.scale = residual_scale, a.eps = eps, a.gate_kind = gate_kind;
+    a.scale = residual_scale, a.eps = eps, a.one_over_cols = (float)(1.0 / (double)cols), a.gate_kind = gate_kind;
     a.post_norm = post_norm != 0, a.pre_norm = pre_norm != 0, a.gains_f32 = gains_dtype == ZKB_F32, a.want_gate = d_dgate != nullptr;
     if (!(a.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
-    if (dtype == ZKB_F32) return norm_backward_dispatch<float>(a, wide, d_dpost_gain, d_dpre_gain, s);
-    if (dtype == ZKB_F16) return norm_backward_dispatch<__half>(a, wide, d_dpost_gain, d_dpre_gain, s);
-    return norm_backward_dispatch<bf16>(a, wide, d_dpost_gain, d_dpre_gain, s);
+    if (dtype == ZKB_F32) return wide ? norm_backward_launch<float, true>(a, d_dpost_gain, d_dpre_gain, s) : norm_backward_launch<float, false>(a, d_dpost_gain, d_dpre_gain, s);
+    if (dtype == ZKB_F16) return wide ? norm_backward_launch<__half, true>(a, d_dpost_gain, d_dpre_gain, s) : norm_backward_launch<__half, false>(a, d_dpost_gain, d_dpre_gain, s);
+    return wide ? norm_backward_launch<bf16, true>(a, d_dpost_gain, d_dpre_gain, s) : norm_backward_launch<bf16, false>(a, d_dpost_gain, d_dpre_gain, s);
 }
 
 }  // extern "C"
