@@ -93,7 +93,9 @@ struct RowRing {
             }
     }
     __device__ __forceinline__ void wait(unsigned slot, uint32_t parity) const { tc::barrier_wait(bars + 8 * slot, parity, watch); }
-    __device__ __forceinline__ uint32_t row_of(int k, size_t row, unsigned slot) const {   // in shared memory
+    // in shared memory
+    template <bool kAligned> __device__ __forceinline__ uint32_t row_of(int k, size_t row, unsigned slot) const {
+        if (kAligned) return tc::smem_address(slots) + slot * slot_bytes + src[k].at;
         const unsigned at = (unsigned)reinterpret_cast<unsigned long long>(src[k].p) + (unsigned)row * (unsigned)src[k].ld;
         return tc::smem_address(slots) + slot * slot_bytes + src[k].at + (at & 15);
     }
@@ -224,52 +226,46 @@ __device__ __forceinline__ void load_gain(const void* p, bool f32, const Place<k
     }
 }
 
-// Sums of up to 8 values over the block's threads (whole warps), for every thread.  Within a warp the values are dealt out while they are
-// added, so that eight take nine exchanges and not forty.  `buf`: 8 floats a warp; two calls on it need a barrier between.
-template <int K>
+// Sums of K values (1 or up to 8) over the block's threads (whole warps, kWarps at most), for every thread.  Within a warp the values are
+// dealt out while they are added, so that eight take nine exchanges and not forty.  `buf`: 8 floats a warp; two calls on it need a
+// barrier between.
+template <int kWarps, int K>
 __device__ __forceinline__ void row_sums(float (&v)[K], float* buf) {
-    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    float mine;
-    if constexpr (K == 1) {
-        mine = v[0];
+    constexpr int P = K == 1 ? 1 : 8;
+    const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    float w[P];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0) buf[warp] = mine;
-        __syncthreads();
-        mine = lane < warps ? buf[lane] : 0.0f;
+    for (int k = 0; k < P; ++k) w[k] = k < K ? v[k] : 0.0f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        v[0] = mine;
-    } else {
-        float w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = k < K ? v[k] : 0.0f;
-#pragma unroll
-        for (int o = 16, n = 4; n > 0; o >>= 1, n >>= 1) {
+    for (int o = 16, n = P / 2; o > 0; o >>= 1, n >>= 1) {
+        if (n > 0) {
             const bool up = lane & o;
 #pragma unroll
             for (int k = 0; k < n; ++k) {
                 const float give = up ? w[k] : w[k + n];
                 w[k] = (up ? w[k + n] : w[k]) + __shfl_xor_sync(0xffffffffu, give, o);
             }
+        } else {
+            w[0] += __shfl_xor_sync(0xffffffffu, w[0], o);
         }
-        mine = w[0] + __shfl_xor_sync(0xffffffffu, w[0], 2);
-        mine += __shfl_xor_sync(0xffffffffu, mine, 1);          // value lane / 4 of this warp
-        if ((lane & 3) == 0) buf[warp * 8 + lane / 4] = mine;
-        __syncthreads();
-        mine = 0.0f;
-        for (unsigned i = lane / 8; i < warps; i += 4) mine += buf[i * 8 + lane % 8];
-        mine += __shfl_xor_sync(0xffffffffu, mine, 8);
-        mine += __shfl_xor_sync(0xffffffffu, mine, 16);
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, mine, k);
     }
+    // lane / (32 / P) says which value a lane has the warp's sum of
+    if (lane % (32 / P) == 0) buf[(threadIdx.x >> 5) * P + lane / (32 / P)] = w[0];
+    __syncthreads();
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWarps; i += 32 / P)
+        if (i + lane / P < warps) mine += buf[(i + lane / P) * P + lane % P];
+#pragma unroll
+    for (int o = P; o < 32; o <<= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = P == 1 ? mine : __shfl_sync(0xffffffffu, mine, k);
 }
 
 // How a kernel is laid out.  Slots: rows come through the ring and the values that all rows share (gains, a CHANNEL gate) stay in
 // registers: with the ring in shared memory little first-level cache is left, and read for each row they would come from L2, as many
-// bytes as the rows themselves.  Rows of more than 8192 values take 16 to a thread of 1024 and leave no registers for that, nor
-// is there room for their slots: they read straight from global memory.
+// bytes as the rows themselves.  Rows of more than 8192 values take 16 to a thread of 1024 and leave no registers for that, and
+// some rows leave no room for two slots: they are read straight from global memory.
 template <bool kAligned_, int kShare_, int kThreads_, int kBlocks_, bool kSlots_> struct Layout {
     static constexpr bool kAligned = kAligned_, kSlots = kSlots_;
     static constexpr int kShare = kShare_, kThreads = kThreads_, kBlocks = kBlocks_;
@@ -277,7 +273,7 @@ template <bool kAligned_, int kShare_, int kThreads_, int kBlocks_, bool kSlots_
 template <class T, class L> using From = std::conditional_t<L::kSlots, InSlot<T>, InMemory<T>>;
 template <class T, class L, int N>
 __device__ __forceinline__ From<T, L> row_from(const RowRing<T, N>& ring, const Source* src, int k, size_t row, unsigned slot) {
-    if constexpr (L::kSlots) return {ring.row_of(k, row, slot)};
+    if constexpr (L::kSlots) return {ring.template row_of<L::kAligned>(k, row, slot)};
     else return {reinterpret_cast<const T*>(src[k].p + row * src[k].ld)};
 }
 
@@ -337,7 +333,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_kernel(con
         float post_inv = 1.0f;
         if (a.post_norm) {
             s[0] = total(s2);
-            row_sums<1>(s, sums);
+            row_sums<L::kThreads / 32, 1>(s, sums);
             post_inv = rsqrtf(s[0] * a.one_over_cols + a.eps);
             if (threadIdx.x == 0 && a.post_inv) a.post_inv[row] = post_inv;
         }
@@ -366,7 +362,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_kernel(con
             for (int j = 0; j < G / 2; ++j) s2 = fma(x[g][j], x[g][j], s2);
         }
         s[0] = total(s2);
-        row_sums<1>(s, sums + 32 + 32 * odd);      // behind its barrier every thread has read this row's slot
+        row_sums<L::kThreads / 32, 1>(s, sums + 32 + 32 * odd);      // behind its barrier every thread has read this row's slot
         odd ^= 1;
         if (L::kSlots) {
             const size_t next = row + (size_t)a.slots * gridDim.x;
@@ -494,10 +490,10 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_backward_k
             }
         }
         float s[6] = {total(rr), total(pr), total(yy), total(eyd), total(eyp), total(eyr)};
-        row_sums<6>(s, sums[odd]);
+        row_sums<L::kThreads / 32, 6>(s, sums[odd]);
         odd ^= 1;
         if (L::kSlots) {   // behind the barrier in row_sums every thread is done with the row before
-            if (threadIdx.x == 0 && row >= gridDim.x && a.slots > 1) {
+            if (threadIdx.x == 0 && row >= gridDim.x) {
                 const size_t next = row + (size_t)(a.slots - 1) * gridDim.x;
                 if (next < a.rows) ring.fetch(next, done);
             }
@@ -560,10 +556,6 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_backward_k
                 for (int j = 0; j < G / 2; ++j) d[j] = fma(d[j] * w[j], by2, y[j] * less);
                 store_group<T>(dy_row, at, d);
             }
-        }
-        if (L::kSlots && a.slots == 1) {
-            __syncthreads();
-            if (threadIdx.x == 0 && row + gridDim.x < a.rows) ring.fetch(row + gridDim.x, 0);
         }
     }
     if (!a.partial) return;
@@ -628,25 +620,30 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const __grid_constant_
 unsigned row_threads(size_t cols, unsigned per) { return std::max(32u, div_up(div_up(cols, per), 32) * 32); }
 
 constexpr size_t kRingHead = 16 * 8;
+// Places the matrices in a slot; returns its bytes.
+template <class Args> size_t lay_slot(Args* a, int matrices, size_t es) {
+    size_t slot = 0;
+    for (int k = 0; k < matrices; ++k) {
+        a->src[k].at = (unsigned)slot;
+        if (a->src[k].p) slot += slot_row_bytes(a->cols, es);
+    }
+    a->slot_bytes = (unsigned)slot;
+    return std::max<size_t>(slot, 16);
+}
+// slots of each block's ring; of its share, 1 KB is the system's and up to 3 KB the sums'
+size_t slots_for(size_t slot, int blocks_per_sm) { return std::min<size_t>(8, (224 * 1024 / blocks_per_sm - 4096 - kRingHead) / slot); }
+
 // The grid of a kernel over rows, and its ring: as many blocks as are resident, each with as many slots as fit.
 template <class L, class Kernel, class Args>
-int plan_rows(Kernel kernel, unsigned threads, int matrices, size_t es, Args* a, unsigned* blocks, size_t* smem) {
+int plan_rows(Kernel kernel, unsigned threads, Args* a, unsigned* blocks, size_t* smem) {
     int resident = 0;
     ZKB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, kRingHead));
     resident = std::max(1, resident);
     *smem = kRingHead;
     if (L::kSlots) {
-        size_t slot = 0;
-        for (int k = 0; k < matrices; ++k) {
-            a->src[k].at = (unsigned)slot;
-            if (a->src[k].p) slot += slot_row_bytes(a->cols, es);
-        }
-        a->slot_bytes = (unsigned)slot;
-        slot = std::max<size_t>(slot, 16);
-        const size_t room = 224 * 1024, other = 4096 + kRingHead;   // of each block's share, 1 KB is the system's and up to 3 KB the sums'
-        const auto fit = [&](int blocks_per_sm) { return (room / blocks_per_sm - other) / slot; };
-        while (resident > 1 && fit(resident) < 3) --resident;
-        a->slots = (unsigned)std::min<size_t>(8, std::max<size_t>(1, fit(resident)));
+        const size_t slot = std::max(a->slot_bytes, 16u);
+        while (resident > 1 && slots_for(slot, resident) < 3) --resident;
+        a->slots = (unsigned)slots_for(slot, resident);
         *smem += a->slots * slot;
         ZKB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)*smem));
     }
@@ -660,11 +657,12 @@ int norm_launch(NormArgs a, cudaStream_t s) {
     const auto kernel = block_norm_kernel<T, L>;
     unsigned blocks;
     size_t smem;
-    ZKB_TRY((plan_rows<L>(kernel, threads, 3, sizeof(T), &a, &blocks, &smem)));
+    ZKB_TRY((plan_rows<L>(kernel, threads, &a, &blocks, &smem)));
     return launch_beside("block_norm", kernel, blocks, threads, smem, s, a);
 }
 template <class T, bool kAligned>
-int norm_launch(const NormArgs& a, cudaStream_t s) {
+int norm_launch(NormArgs a, cudaStream_t s) {
+    lay_slot(&a, 3, sizeof(T));
     if (a.cols <= 4096) return norm_launch<T, Layout<kAligned, 8, 512, 2, true>>(a, s);
     if (a.cols <= 8192) return norm_launch<T, Layout<kAligned, 8, 1024, 1, true>>(a, s);
     return norm_launch<T, Layout<kAligned, 16, 1024, 1, false>>(a, s);
@@ -676,7 +674,7 @@ int norm_backward_launch(NormGradArgs a, void* dpost, void* dpre, cudaStream_t s
     const auto kernel = block_norm_backward_kernel<T, L>;
     unsigned blocks;
     size_t smem;
-    ZKB_TRY((plan_rows<L>(kernel, threads, 5, sizeof(T), &a, &blocks, &smem)));
+    ZKB_TRY((plan_rows<L>(kernel, threads, &a, &blocks, &smem)));
     Scratch scratch(s);
     const bool channel = a.want_gate && a.gate_kind == ZKB_GATE_CHANNEL;
     if (dpre || dpost || channel) {
@@ -690,10 +688,11 @@ int norm_backward_launch(NormGradArgs a, void* dpost, void* dpre, cudaStream_t s
     return launch_beside("norm_reduce", norm_reduce_kernel<T>, dim3(div_up(a.cols, 32), 2), 256, 0, s, n);
 }
 template <class T, bool kAligned>
-int norm_backward_launch(const NormGradArgs& a, void* dpost, void* dpre, cudaStream_t s) {
-    if (a.cols <= 2560) return norm_backward_launch<T, Layout<kAligned, 8, 320, 2, true>>(a, dpost, dpre, s);
-    if (a.cols <= 5120) return norm_backward_launch<T, Layout<kAligned, 8, 640, 1, true>>(a, dpost, dpre, s);
-    if (a.cols <= 8192) return norm_backward_launch<T, Layout<kAligned, 16, 512, 1, true>>(a, dpost, dpre, s);
+int norm_backward_launch(NormGradArgs a, void* dpost, void* dpre, cudaStream_t s) {
+    const bool slots = slots_for(lay_slot(&a, 5, sizeof(T)), 1) >= 2;   // the present row and one on its way
+    if (slots && a.cols <= 2560) return norm_backward_launch<T, Layout<kAligned, 8, 320, 2, true>>(a, dpost, dpre, s);
+    if (slots && a.cols <= 5120) return norm_backward_launch<T, Layout<kAligned, 8, 640, 1, true>>(a, dpost, dpre, s);
+    if (slots && a.cols <= 8192) return norm_backward_launch<T, Layout<kAligned, 16, 512, 1, true>>(a, dpost, dpre, s);
     return norm_backward_launch<T, Layout<kAligned, 16, 1024, 1, false>>(a, dpost, dpre, s);
 }
 

@@ -19,6 +19,7 @@ struct RopeTensor {
     void* out;
     long long ib, it, ih, ob, ot, oh;
     unsigned first_head;   // heads of the tensors before this one
+    unsigned heads;
     bool copy_tail;        // out is not in: the values behind the turned ones have to be brought over
 };
 struct RopeArgs {
@@ -33,7 +34,8 @@ struct RopeArgs {
 // Bound by HBM: each value is read and written once.  A block takes a few tokens: their sines and cosines are formed once,
 // in shared memory, and serve every head of every tensor.  The angle is reduced to a fraction of a turn in 64 bits (a
 // 32-bit product is off by 0.01 radians at position 131072) and only the fraction is rounded to 32.
-// P pairs make a unit of work, in 16-byte vectors where sizes, strides and addresses allow it, else one pair at a time.
+// P pairs make a unit of work, in 16-byte vectors where sizes, strides and addresses allow it, else one pair at a time.  A thread
+// keeps its unit and goes through the heads, four at a time so that their loads are in flight together.
 template <class T, bool kWidePath, bool kInterleaved>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
     extern __shared__ float2 turn[];
@@ -52,55 +54,75 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
 
     constexpr int V = kWidePath ? kWide<T> : 1;
     constexpr int P = kWidePath && kInterleaved ? V / 2 : V;
-    const unsigned turned = a.half / P;                    // P divides half
+    constexpr int N = kWidePath && !kInterleaved ? 2 : 1;   // vectors of a unit
+    const unsigned turned = a.half / P;                     // P divides half
     const unsigned units = turned + a.tail / V;
-    const unsigned heads_here = (a.heads + gridDim.y - 1) / gridDim.y;
-    const unsigned head0 = blockIdx.y * heads_here;
-    const unsigned n_heads = head0 < a.heads ? min(heads_here, a.heads - head0) : 0;
-    for (unsigned i = threadIdx.x; i < n_tok * n_heads * units; i += kRopeThreads) {
-        const unsigned row = i / units, u = i % units;
-        const unsigned tl = row / n_heads;
-        unsigned h = head0 + row % n_heads, k = 0;
-        while (k + 1 < a.n_tensors && h >= a.t[k + 1].first_head) ++k;
-        const RopeTensor& x = a.t[k];
-        h -= x.first_head;
+    const unsigned side = min(units, (unsigned)kRopeThreads), lanes = kRopeThreads / side;   // threads to a head, heads at a time
+    if (threadIdx.x >= side * lanes) return;
+    const unsigned heads_here = (a.heads + gridDim.y - 1) / gridDim.y, head0 = blockIdx.y * heads_here;
+    const unsigned head1 = min(head0 + heads_here, a.heads), mine = threadIdx.x / side;
+    for (unsigned tl = 0; tl < n_tok; ++tl) {
         const unsigned t = tok0 + tl, b = t / a.tokens, s = t % a.tokens;
-        const T* in = static_cast<const T*>(x.in) + b * x.ib + s * x.it + h * x.ih;
-        T* out = static_cast<T*>(x.out) + b * x.ob + s * x.ot + h * x.oh;
-        if (u >= turned) {
-            if (x.copy_tail) {
-                const unsigned at = 2 * a.half + (u - turned) * V;
-                *reinterpret_cast<Vec<T, V>*>(out + at) = *reinterpret_cast<const Vec<T, V>*>(in + at);
+        for (unsigned k = 0; k < a.n_tensors; ++k) {
+            const RopeTensor& x = a.t[k];
+            const unsigned begin = max(head0, x.first_head), end = min(head1, x.first_head + x.heads);
+            if (begin >= end) continue;
+            const T* const in0 = static_cast<const T*>(x.in) + b * x.ib + s * x.it;
+            T* const out0 = static_cast<T*>(x.out) + b * x.ob + s * x.ot;
+            for (unsigned u = threadIdx.x % side; u < units; u += side) {
+                const bool copy = u >= turned;
+                if (copy && !x.copy_tail) continue;
+                // where the unit's first and second values of its pairs begin
+                const unsigned lo = copy ? 2 * a.half + (u - turned) * V : kInterleaved ? 2 * P * u : P * u;
+                const unsigned hi = kInterleaved ? lo + 1 : a.half + lo;
+                float2 cs[P];
+#pragma unroll
+                for (int j = 0; j < P; ++j) cs[j] = copy ? make_float2(1.0f, 0.0f) : turn[tl * a.half + u * P + j];
+                for (unsigned h = begin + mine; h < end; h += 4 * lanes) {
+                    Vec<T, V> v[4][N];
+                    T second[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const unsigned g = h + q * lanes;
+                        if (g >= end) continue;
+                        const T* in = in0 + (long long)(g - x.first_head) * x.ih;
+                        v[q][0] = *reinterpret_cast<const Vec<T, V>*>(in + lo);
+                        if constexpr (N == 2) {
+                            if (!copy) v[q][1] = *reinterpret_cast<const Vec<T, V>*>(in + hi);
+                        }
+                        if constexpr (!kWidePath) {
+                            if (!copy) second[q] = in[hi];
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const unsigned g = h + q * lanes;
+                        if (g >= end) continue;
+                        T* out = out0 + (long long)(g - x.first_head) * x.oh;
+                        if (copy) {
+                            *reinterpret_cast<Vec<T, V>*>(out + lo) = v[q][0];
+                            continue;
+                        }
+                        Vec<T, V> w[N];
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            const float x0 = to_f32<T>(kWidePath && kInterleaved ? v[q][0].v[2 * j] : v[q][0].v[j]);
+                            const float x1 = to_f32<T>(!kWidePath ? second[q] : kInterleaved ? v[q][0].v[(2 * j + 1) % V] : v[q][N - 1].v[j]);
+                            const T y0 = from_f32<T>(x0 * cs[j].x - x1 * cs[j].y), y1 = from_f32<T>(x1 * cs[j].x + x0 * cs[j].y);
+                            if constexpr (kWidePath && kInterleaved) {
+                                w[0].v[2 * j] = y0;
+                                w[0].v[2 * j + 1] = y1;
+                            } else {
+                                w[0].v[j] = y0;
+                                if constexpr (kWidePath) w[1].v[j] = y1;
+                                else out[hi] = y1;
+                            }
+                        }
+                        *reinterpret_cast<Vec<T, V>*>(out + lo) = w[0];
+                        if constexpr (N == 2) *reinterpret_cast<Vec<T, V>*>(out + hi) = w[1];
+                    }
+                }
             }
-            continue;
-        }
-        const float2* cs = turn + tl * a.half + u * P;
-        constexpr int stride = kInterleaved ? 2 : 1;
-        float lo[P], hi[P];
-        if constexpr (kWidePath && kInterleaved) {
-            float v[V];
-            load_vec<T, V>(in + u * V, v);
-#pragma unroll
-            for (int j = 0; j < P; ++j) { lo[j] = v[2 * j]; hi[j] = v[2 * j + 1]; }
-        } else {
-            load_vec<T, P>(in + stride * u * P, lo);
-            load_vec<T, P>(in + (kInterleaved ? 2 * u + 1 : a.half + u * P), hi);
-        }
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const float2 c = cs[j];
-            const float x0 = lo[j], x1 = hi[j];
-            lo[j] = x0 * c.x - x1 * c.y;
-            hi[j] = x1 * c.x + x0 * c.y;
-        }
-        if constexpr (kWidePath && kInterleaved) {
-            float v[V];
-#pragma unroll
-            for (int j = 0; j < P; ++j) { v[2 * j] = lo[j]; v[2 * j + 1] = hi[j]; }
-            store_vec<T, V>(out + u * V, v);
-        } else {
-            store_vec<T, P>(out + stride * u * P, lo);
-            store_vec<T, P>(out + (kInterleaved ? 2 * u + 1 : a.half + u * P), hi);
         }
     }
 }
@@ -194,7 +216,7 @@ int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, 
         for (unsigned j = 0; j < a.n_tensors; ++j)
             if (a.t[j].out == h.d_out) return fail(ZKB_ERR_ARG, "zkb_rope: two tensors with one output");
         RopeTensor& x = a.t[a.n_tensors++];
-        x = {h.d_in, h.d_out, h.in_batch, h.in_token, h.in_head, h.out_batch, h.out_token, h.out_head, a.heads, !same};
+        x = {h.d_in, h.d_out, h.in_batch, h.in_token, h.in_head, h.out_batch, h.out_token, h.out_head, a.heads, (unsigned)h.heads, !same};
         a.heads += (unsigned)h.heads;
         const long long strides[6] = {x.ib, x.it, x.ih, x.ob, x.ot, x.oh};
         for (long long st : strides) wide = wide && st % (long long)v == 0;
