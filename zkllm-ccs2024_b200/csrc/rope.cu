@@ -12,19 +12,18 @@ namespace zkb {
 namespace {
 
 constexpr int kMaxTensors = 4;
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
 struct RopeTensor {
     const void* in;
     void* out;
     long long ib, it, ih, ob, ot, oh;
-    unsigned first_head;   // heads of the tensors before this one
     unsigned heads;
     bool copy_tail;        // out is not in: the values behind the turned ones have to be brought over
 };
 struct RopeArgs {
     RopeTensor t[kMaxTensors];
-    unsigned n_tensors, heads, batch_tokens, tokens, half, tail, tokens_per_block;
+    unsigned n_tensors, heads /* the most of a tensor */, batch_tokens, tokens, half, tail, tokens_per_block;
     const double* inv_freq;
     float magnitude, sin_sign;
     const long long* positions;
@@ -32,13 +31,14 @@ struct RopeArgs {
 };
 
 // Bound by HBM: each value is read and written once.  A block takes a few tokens: their sines and cosines are formed once,
-// in shared memory, and serve every head of every tensor.  The angle is reduced to a fraction of a turn in 64 bits (a
+// in shared memory, and serve every head of a tensor (blockIdx.z).  The angle is reduced to a fraction of a turn in 64 bits (a
 // 32-bit product is off by 0.01 radians at position 131072) and only the fraction is rounded to 32.
 // P pairs make a unit of work, in 16-byte vectors where sizes, strides and addresses allow it, else one pair at a time.  A thread
-// keeps its unit and goes through the heads, four at a time so that their loads are in flight together.
+// keeps its unit and goes through the heads of the block's tokens, kAhead at a time so that their loads are in flight together.
 template <class T, bool kWidePath, bool kInterleaved>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const __grid_constant__ RopeArgs a) {
     extern __shared__ float2 turn[];
+    const RopeTensor& x = a.t[blockIdx.z];
     const unsigned tok0 = blockIdx.x * a.tokens_per_block;
     const unsigned n_tok = min(a.tokens_per_block, a.batch_tokens - tok0);
     for (unsigned i = threadIdx.x; i < n_tok * a.half; i += kRopeThreads) {
@@ -59,69 +59,63 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     const unsigned units = turned + a.tail / V;
     const unsigned side = min(units, (unsigned)kRopeThreads), lanes = kRopeThreads / side;   // threads to a head, heads at a time
     if (threadIdx.x >= side * lanes) return;
-    const unsigned heads_here = (a.heads + gridDim.y - 1) / gridDim.y, head0 = blockIdx.y * heads_here;
-    const unsigned head1 = min(head0 + heads_here, a.heads), mine = threadIdx.x / side;
-    for (unsigned tl = 0; tl < n_tok; ++tl) {
-        const unsigned t = tok0 + tl, b = t / a.tokens, s = t % a.tokens;
-        for (unsigned k = 0; k < a.n_tensors; ++k) {
-            const RopeTensor& x = a.t[k];
-            const unsigned begin = max(head0, x.first_head), end = min(head1, x.first_head + x.heads);
-            if (begin >= end) continue;
-            const T* const in0 = static_cast<const T*>(x.in) + b * x.ib + s * x.it;
-            T* const out0 = static_cast<T*>(x.out) + b * x.ob + s * x.ot;
-            for (unsigned u = threadIdx.x % side; u < units; u += side) {
-                const bool copy = u >= turned;
-                if (copy && !x.copy_tail) continue;
-                // where the unit's first and second values of its pairs begin
-                const unsigned lo = copy ? 2 * a.half + (u - turned) * V : kInterleaved ? 2 * P * u : P * u;
-                const unsigned hi = kInterleaved ? lo + 1 : a.half + lo;
-                float2 cs[P];
+    const unsigned heads_here = (x.heads + gridDim.y - 1) / gridDim.y, head0 = blockIdx.y * heads_here;
+    const unsigned n_heads = head0 < x.heads ? min(heads_here, x.heads - head0) : 0, rows = n_tok * n_heads;
+    constexpr int kAhead = 2;
+    for (unsigned u = threadIdx.x % side; u < units; u += side) {
+        const bool copy = u >= turned;
+        if (copy && !x.copy_tail) break;
+        // where the unit's first and second values of its pairs begin
+        const unsigned lo = copy ? 2 * a.half + (u - turned) * V : kInterleaved ? 2 * P * u : P * u;
+        const unsigned hi = kInterleaved ? lo + 1 : a.half + lo;
+        for (unsigned r0 = threadIdx.x / side; r0 < rows; r0 += kAhead * lanes) {
+            Vec<T, V> v[kAhead][N];
+            T second[kAhead], *to[kAhead];
+            unsigned token[kAhead];
 #pragma unroll
-                for (int j = 0; j < P; ++j) cs[j] = copy ? make_float2(1.0f, 0.0f) : turn[tl * a.half + u * P + j];
-                for (unsigned h = begin + mine; h < end; h += 4 * lanes) {
-                    Vec<T, V> v[4][N];
-                    T second[4];
+            for (int q = 0; q < kAhead; ++q) {
+                const unsigned r = r0 + q * lanes;
+                to[q] = nullptr;
+                if (r >= rows) continue;
+                token[q] = r / n_heads;
+                const unsigned h = head0 + r - token[q] * n_heads, t = tok0 + token[q], b = t / a.tokens, s = t - b * a.tokens;
+                const T* in = static_cast<const T*>(x.in) + (b * x.ib + s * x.it + h * x.ih);
+                to[q] = static_cast<T*>(x.out) + (b * x.ob + s * x.ot + h * x.oh);
+                v[q][0] = *reinterpret_cast<const Vec<T, V>*>(in + lo);
+                if constexpr (N == 2) {
+                    if (!copy) v[q][1] = *reinterpret_cast<const Vec<T, V>*>(in + hi);
+                }
+                if constexpr (!kWidePath) {
+                    if (!copy) second[q] = in[hi];
+                }
+            }
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const unsigned g = h + q * lanes;
-                        if (g >= end) continue;
-                        const T* in = in0 + (long long)(g - x.first_head) * x.ih;
-                        v[q][0] = *reinterpret_cast<const Vec<T, V>*>(in + lo);
-                        if constexpr (N == 2) {
-                            if (!copy) v[q][1] = *reinterpret_cast<const Vec<T, V>*>(in + hi);
-                        }
-                        if constexpr (!kWidePath) {
-                            if (!copy) second[q] = in[hi];
-                        }
-                    }
+            for (int q = 0; q < kAhead; ++q) {
+                T* const out = to[q];
+                if (!out) continue;
+                if (copy) {
+                    *reinterpret_cast<Vec<T, V>*>(out + lo) = v[q][0];
+                    continue;
+                }
+                const float2* cs = turn + token[q] * a.half + u * P;
+                Vec<T, V> w[N];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const unsigned g = h + q * lanes;
-                        if (g >= end) continue;
-                        T* out = out0 + (long long)(g - x.first_head) * x.oh;
-                        if (copy) {
-                            *reinterpret_cast<Vec<T, V>*>(out + lo) = v[q][0];
-                            continue;
-                        }
-                        Vec<T, V> w[N];
-#pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            const float x0 = to_f32<T>(kWidePath && kInterleaved ? v[q][0].v[2 * j] : v[q][0].v[j]);
-                            const float x1 = to_f32<T>(!kWidePath ? second[q] : kInterleaved ? v[q][0].v[(2 * j + 1) % V] : v[q][N - 1].v[j]);
-                            const T y0 = from_f32<T>(x0 * cs[j].x - x1 * cs[j].y), y1 = from_f32<T>(x1 * cs[j].x + x0 * cs[j].y);
-                            if constexpr (kWidePath && kInterleaved) {
-                                w[0].v[2 * j] = y0;
-                                w[0].v[2 * j + 1] = y1;
-                            } else {
-                                w[0].v[j] = y0;
-                                if constexpr (kWidePath) w[1].v[j] = y1;
-                                else out[hi] = y1;
-                            }
-                        }
-                        *reinterpret_cast<Vec<T, V>*>(out + lo) = w[0];
-                        if constexpr (N == 2) *reinterpret_cast<Vec<T, V>*>(out + hi) = w[1];
+                for (int j = 0; j < P; ++j) {
+                    const float2 c = cs[j];
+                    const float x0 = to_f32<T>(kWidePath && kInterleaved ? v[q][0].v[2 * j] : v[q][0].v[j]);
+                    const float x1 = to_f32<T>(!kWidePath ? second[q] : kInterleaved ? v[q][0].v[(2 * j + 1) % V] : v[q][N - 1].v[j]);
+                    const T y0 = from_f32<T>(x0 * c.x - x1 * c.y), y1 = from_f32<T>(x1 * c.x + x0 * c.y);
+                    if constexpr (kWidePath && kInterleaved) {
+                        w[0].v[2 * j] = y0;
+                        w[0].v[2 * j + 1] = y1;
+                    } else {
+                        w[0].v[j] = y0;
+                        if constexpr (kWidePath) w[N - 1].v[j] = y1;
+                        else out[hi] = y1;
                     }
                 }
+                *reinterpret_cast<Vec<T, V>*>(out + lo) = w[0];
+                if constexpr (N == 2) *reinterpret_cast<Vec<T, V>*>(out + hi) = w[1];
             }
         }
     }
@@ -129,13 +123,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
 
 template <class T>
 int rope_launch(RopeArgs a, bool interleaved, bool wide, cudaStream_t s) {
-    a.tokens_per_block = a.half >= 512 ? 1 : std::min(8u, 512 / a.half);
+    a.tokens_per_block = a.half >= 512 ? 1 : std::min(4u, 512 / a.half);
     // few tokens: fewer to a block, then the heads over several blocks, until every SM has work
     const unsigned target = 2 * sm_count();
-    while (a.tokens_per_block > 1 && div_up(a.batch_tokens, a.tokens_per_block) < target) a.tokens_per_block >>= 1;
+    while (a.tokens_per_block > 1 && div_up(a.batch_tokens, a.tokens_per_block) * a.n_tensors < target) a.tokens_per_block >>= 1;
     const unsigned gx = div_up(a.batch_tokens, a.tokens_per_block);
-    const unsigned gy = gx >= target ? 1 : std::min(a.heads, target / gx);
-    const dim3 grid(gx, gy);
+    const unsigned gy = gx * a.n_tensors >= target ? 1 : std::min(a.heads, target / (gx * a.n_tensors));
+    const dim3 grid(gx, gy, a.n_tensors);
     const size_t smem = sizeof(float2) * a.tokens_per_block * a.half;
     const auto rope = interleaved ? (wide ? rope_kernel<T, true, true> : rope_kernel<T, false, true>)
                                   : (wide ? rope_kernel<T, true, false> : rope_kernel<T, false, false>);
@@ -216,8 +210,8 @@ int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, 
         for (unsigned j = 0; j < a.n_tensors; ++j)
             if (a.t[j].out == h.d_out) return fail(ZKB_ERR_ARG, "zkb_rope: two tensors with one output");
         RopeTensor& x = a.t[a.n_tensors++];
-        x = {h.d_in, h.d_out, h.in_batch, h.in_token, h.in_head, h.out_batch, h.out_token, h.out_head, a.heads, (unsigned)h.heads, !same};
-        a.heads += (unsigned)h.heads;
+        x = {h.d_in, h.d_out, h.in_batch, h.in_token, h.in_head, h.out_batch, h.out_token, h.out_head, (unsigned)h.heads, !same};
+        a.heads = std::max(a.heads, (unsigned)h.heads);
         const long long strides[6] = {x.ib, x.it, x.ih, x.ob, x.ot, x.oh};
         for (long long st : strides) wide = wide && st % (long long)v == 0;
         wide = wide && aligned_to(h.d_in, 16) && aligned_to(h.d_out, 16);
