@@ -34,17 +34,21 @@ __device__ __forceinline__ float activate(int kind, float g, float* d) {
 
 // ---- the product kernel -----------------------------------------------------------------------------------------------------
 //
-// One persistent block per SM works through 128 x kCols tiles.  Warp 0 copies 64-deep slices of both operands into a ring in
-// shared memory, warp 1 issues the products (128 x kCols x 16 each) into one of two accumulators in tensor memory, warps 4 to 7 take the
-// other accumulator out, so that a tile's epilogue runs beside the next tile's products.
+// Bound by the tensor cores.  Persistent pairs of blocks (one block per SM) work through 256 x 256 tiles.  Each block holds 128 rows of the
+// first operand and 128 columns of the second, so that a slice costs both SMs together 64 KB of copies and shared memory where two
+// blocks on their own would need 96.  In each block warp 0 copies 64-deep slices into a ring; in the first, warp 1 issues
+// the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 7 of both take their 128 rows of the other
+// accumulator out, so that a tile's epilogue runs beside the next tile's products.
 enum Form {
-    kGated,    // A x; B the two weights side by side, kCols / 2 columns of each in a tile; result act(g) * u
+    kGated,    // A x; B the two weights side by side, 128 columns of each in a tile; result act(g) * u
     kSummed,   // A dg then du; B w_gate then w_up: one sum over both; result dx
     kPaired    // A x^T; B dg for the first half of the tiles, du for the second; results dw_gate and dw_up
 };
-constexpr int kRows = 128, kDepth = 64;
+constexpr int kTile = 256, kHalf = 128, kDepth = 64;
 constexpr int kProductThreads = 256;
 constexpr int kStageBytes = 32 * 80;   // an epilogue warp's 32 x 32 values on their way out, rows 80 bytes apart
+constexpr int kRing = 6, kSlice = 2 * kHalf * kDepth * 2;
+constexpr size_t kProductSmem = 1024 + (size_t)kRing * kSlice + 4 * kStageBytes + 256;
 
 struct ProductArgs {
     CUtensorMap a[2], b[2];
@@ -56,11 +60,6 @@ struct ProductArgs {
     int act;
     int* flag;
 };
-
-template <int kCols> constexpr int kRing = kCols == 256 ? 4 : 3;
-template <int kCols> constexpr size_t product_smem() {
-    return 1024 + (size_t)kRing<kCols> * (kRows + kCols) * kDepth * 2 + 4 * kStageBytes + 256;
-}
 
 // 32 x 32 values of a warp (row i with lane i) to rows row0.. and columns col0.. of a matrix of m x n.
 template <class T>
@@ -104,89 +103,86 @@ __device__ __forceinline__ void tile_place(unsigned tile, unsigned row_tiles, un
     *col = in / height;
 }
 
-template <class T, int kForm, int kCols>
-__global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __grid_constant__ ProductArgs p) {
+template <class T, int kForm>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu_product_kernel(const __grid_constant__ ProductArgs p) {
     constexpr bool kAMn = kForm == kPaired, kBMn = kForm != kSummed;
-    constexpr int kA = kRows * kDepth * 2, kB = kCols * kDepth * 2, kSlice = kA + kB, kR = kRing<kCols>;
-    constexpr uint32_t kInstruction = tc::instruction<T>(kRows, kCols, kAMn, kBMn);
+    constexpr int kA = kHalf * kDepth * 2;
+    constexpr uint32_t kInstruction = tc::instruction<T>(kTile, kTile, kAMn, kBMn);
     constexpr int kSums = kForm == kSummed ? 2 : 1;
     extern __shared__ char raw[];
     char* ring = raw + ((1024 - (tc::smem_address(raw) & 1023)) & 1023);
-    char* stages = ring + kR * kSlice;
+    char* stages = ring + kRing * kSlice;
     uint64_t* bars = reinterpret_cast<uint64_t*>(stages + 4 * kStageBytes);
-    volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kR + 5);
-    const uint32_t full = tc::smem_address(bars), empty = full + 8 * kR, ready = empty + 8 * kR, taken = ready + 16, drained = taken + 16;
-    const uint32_t tmem_at = drained + 16;
-    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kRing + 4);
+    const uint32_t full = tc::smem_address(bars), empty = full + 8 * kRing, ready = empty + 8 * kRing, taken = ready + 16;
+    const uint32_t tmem_at = taken + 24;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = tc::cluster_rank();
     const tc::Watch watch = {dead, p.flag};
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kR; ++i) {
+        for (int i = 0; i < kRing; ++i) {
             tc::barrier_init(full + 8 * i, 1);
             tc::barrier_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::barrier_init(ready + 8 * i, 1);
-            tc::barrier_init(taken + 8 * i, 4);
+            tc::barrier_init(taken + 8 * i, 8);   // the epilogue warps of both blocks
         }
-        tc::barrier_init(drained, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc::prefetch_map(&p.a[0]);
         tc::prefetch_map(&p.b[0]);
     }
-    if (warp == 2) tc::tmem_alloc(tmem_at, 2 * kCols);
+    if (warp == 2) tc::tmem_alloc_pair(tmem_at, 2 * kTile);
     tc::fence_before_sync();
     __syncthreads();
+    tc::cluster_barrier();
     tc::fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kRing + 5);
     grid_release();
     grid_wait();
 
     const unsigned tiles = p.row_tiles * p.col_tiles, all = kForm == kPaired ? 2 * tiles : tiles;
-    const unsigned slices = p.slices * kSums;
+    const unsigned slices = p.slices * kSums, first = blockIdx.x / 2, step = gridDim.x / 2;
     if (warp == 0 && lane == 0) {
-        unsigned at = 0, issued = 0;
+        unsigned at = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (unsigned t = blockIdx.x; t < all && fine; t += gridDim.x) {
+        for (unsigned t = first; t < all && fine; t += step) {
             unsigned row, col;
             tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
             const unsigned pair = t / tiles;
             for (unsigned s = 0; s < slices; ++s) {
                 if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
-                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = full + 8 * at;
-                tc::barrier_expect(bar, kSlice);
-                ++issued;
+                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = tc::address_in(full + 8 * at, 0);
+                if (rank == 0) tc::barrier_expect(full + 8 * at, 2 * kSlice);
                 const int sum = kForm == kSummed ? (int)(s / p.slices) : 0;
-                const int k = (int)(s - sum * p.slices) * kDepth;
+                const int k = (int)(s - sum * p.slices) * kDepth, m = row * kTile + rank * kHalf, n = col * kTile + rank * kHalf;
                 if constexpr (kAMn) {
-                    for (int i = 0; i < kRows / 64; ++i) tc::load_box(&p.a[0], a + i * 8192, bar, row * kRows + i * 64, k);
+                    tc::load_box_pair(&p.a[0], a, bar, m, k);
+                    tc::load_box_pair(&p.a[0], a + 8192, bar, m + 64, k);
                 } else {
-                    tc::load_box(&p.a[sum], a, bar, k, row * kRows);
+                    tc::load_box_pair(&p.a[sum], a, bar, k, m);
                 }
-                if constexpr (kForm == kGated) {
-                    for (int i = 0; i < kCols / 128; ++i) {
-                        tc::load_box(&p.b[0], b + i * 8192, bar, col * (kCols / 2) + i * 64, k);
-                        tc::load_box(&p.b[1], b + (kCols / 128 + i) * 8192, bar, col * (kCols / 2) + i * 64, k);
-                    }
+                if constexpr (kForm == kGated) {   // the first block holds w_gate's columns, the second w_up's
+                    tc::load_box_pair(&p.b[rank], b, bar, col * kHalf, k);
+                    tc::load_box_pair(&p.b[rank], b + 8192, bar, col * kHalf + 64, k);
                 } else if constexpr (kForm == kPaired) {
-                    for (int i = 0; i < kCols / 64; ++i) tc::load_box(&p.b[pair], b + i * 8192, bar, col * kCols + i * 64, k);
+                    tc::load_box_pair(&p.b[pair], b, bar, n, k);
+                    tc::load_box_pair(&p.b[pair], b + 8192, bar, n + 64, k);
                 } else {
-                    tc::load_box(&p.b[sum], b, bar, k, col * kCols);
+                    tc::load_box_pair(&p.b[sum], b, bar, k, n);
                 }
-                if (++at == kR) { at = 0; phase ^= 1; }
+                if (++at == kRing) { at = 0; phase ^= 1; }
             }
         }
-        if (!fine)   // the copies in flight write to this block's memory: it ends after them
-            for (unsigned i = issued > kR ? issued - kR : 0; i < issued; ++i) tc::barrier_wait(full + 8 * (i % kR), (i / kR) & 1, watch, true);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
         unsigned at = 0, count = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (unsigned t = blockIdx.x; t < all && fine; t += gridDim.x, ++count) {
+        for (unsigned t = first; t < all && fine; t += step, ++count) {
             const unsigned acc = count & 1;
-            if (!tc::barrier_wait(taken + 8 * acc, ((count >> 1) & 1) ^ 1, watch)) { fine = false; break; }
+            if (!tc::barrier_wait(taken + 8 * acc, ((count >> 1) & 1) ^ 1, watch)) break;
             tc::fence_after_sync();
             for (unsigned s = 0; s < slices; ++s) {
                 if (!tc::barrier_wait(full + 8 * at, phase, watch)) { fine = false; break; }
@@ -194,35 +190,31 @@ __global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __gr
                 const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA;
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; ++k)
-                    tc::product(tmem + acc * kCols, tc::tile_descriptor(a + k * (kAMn ? 2048 : 32), kAMn, 8192),
-                                tc::tile_descriptor(b + k * (kBMn ? 2048 : 32), kBMn, 8192), kInstruction, s || k);
-                tc::commit(empty + 8 * at);
-                if (++at == kR) { at = 0; phase ^= 1; }
+                    tc::product_pair(tmem + acc * kTile, tc::tile_descriptor(a + k * (kAMn ? 2048 : 32), kAMn, 8192),
+                                     tc::tile_descriptor(b + k * (kBMn ? 2048 : 32), kBMn, 8192), kInstruction, s || k);
+                tc::commit_pair(empty + 8 * at);
+                if (++at == kRing) { at = 0; phase ^= 1; }
             }
-            if (fine) tc::commit(ready + 8 * acc);
-        }
-        if (!fine) {   // products in flight read this block's memory
-            tc::commit(drained);
-            tc::barrier_wait(drained, 0, watch, true);
+            if (fine) tc::commit_pair(ready + 8 * acc);
         }
     } else if (warp >= 4) {
         char* stage = stages + (warp - 4) * kStageBytes;
         unsigned count = 0;
-        for (unsigned t = blockIdx.x; t < all; t += gridDim.x, ++count) {
+        for (unsigned t = first; t < all; t += step, ++count) {
             unsigned row, col;
             tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
             const unsigned acc = count & 1, pair = t / tiles;
             const bool fine = tc::barrier_wait(ready + 8 * acc, (count >> 1) & 1, watch);
             if (!__all_sync(0xffffffffu, fine)) break;
             tc::fence_after_sync();
-            const uint32_t from = tmem + ((warp - 4) * 32 << 16) + acc * kCols;
-            const unsigned row0 = row * kRows + (warp - 4) * 32;
+            const uint32_t from = tmem + ((warp - 4) * 32 << 16) + acc * kTile;
+            const unsigned row0 = row * kTile + rank * kHalf + (warp - 4) * 32;
             if constexpr (kForm == kGated) {
-                for (int c = 0; c < kCols / 2; c += 32) {
+                for (int c = 0; c < kHalf; c += 32) {
                     float g[32], u[32];
                     tc::load_columns(from + c, g);
-                    tc::load_columns(from + kCols / 2 + c, u);
-                    const unsigned col0 = col * (kCols / 2) + c;
+                    tc::load_columns(from + kHalf + c, u);
+                    const unsigned col0 = col * kHalf + c;
                     if (p.out[1]) {
                         store_block<T>(stage, g, static_cast<T*>(p.out[1]), p.ld[1], p.wide[1], row0, col0, p.m, p.n);
                         store_block<T>(stage, u, static_cast<T*>(p.out[2]), p.ld[2], p.wide[2], row0, col0, p.m, p.n);
@@ -232,23 +224,25 @@ __global__ void __launch_bounds__(kProductThreads) glu_product_kernel(const __gr
                     store_block<T>(stage, g, static_cast<T*>(p.out[0]), p.ld[0], p.wide[0], row0, col0, p.m, p.n);
                 }
             } else {
-                for (int c = 0; c < kCols; c += 32) {
+                for (int c = 0; c < kTile; c += 32) {
                     float v[32];
                     tc::load_columns(from + c, v);
-                    store_block<T>(stage, v, static_cast<T*>(p.out[pair]), p.ld[pair], p.wide[pair], row0, col * kCols + c, p.m, p.n);
+                    store_block<T>(stage, v, static_cast<T*>(p.out[pair]), p.ld[pair], p.wide[pair], row0, col * kTile + c, p.m, p.n);
                 }
             }
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) tc::barrier_arrive(taken + 8 * acc);
+            if (lane == 0) tc::barrier_arrive_in(tc::address_in(taken + 8 * acc, 0));
         }
     }
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
+    if (*dead) tc::pause();   // a wait ran out: what is in flight between the two blocks lands before either ends
+    tc::cluster_barrier();
     if (warp == 2) {
         tc::fence_after_sync();
-        tc::tmem_free(tmem, 2 * kCols);
+        tc::tmem_free_pair(tmem, 2 * kTile);
     }
 }
 
@@ -495,25 +489,15 @@ int align(Operand* x, size_t rows, size_t cols, Scratch* scratch, cudaStream_t s
     return ZKB_OK;
 }
 
-template <class T, int kForm, int kCols>
+template <class T, int kForm>
 int product_launch(const ProductArgs& p, cudaStream_t s) {
-    const auto glu_product = glu_product_kernel<T, kForm, kCols>;
-    constexpr size_t smem = product_smem<kCols>();
-    ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const auto glu_product = glu_product_kernel<T, kForm>;
+    ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kProductSmem));
     const unsigned tiles = p.row_tiles * p.col_tiles * (kForm == kPaired ? 2 : 1);
-    return launch_beside("glu_product", glu_product, std::min(tiles, (kCols == 256 ? 1u : 2u) * sm_count()), kProductThreads, smem, s, p);
+    return launch_beside("glu_product", glu_product, 2 * std::min(tiles, (unsigned)sm_count() / 2), kProductThreads, kProductSmem, s, p);
 }
 
 template <class T> constexpr int kCode = std::is_same<T, __half>::value ? ZKB_F16 : ZKB_BF16;
-
-template <class T, int kCols>
-int glu_forward(const GluArgs& a, Operand x, Operand wg, Operand wu, ProductArgs& p, cudaStream_t s) {
-    ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kRows));
-    ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
-    ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
-    p.row_tiles = div_up(a.tokens, kRows), p.col_tiles = div_up(a.hidden, kCols / 2);
-    return product_launch<T, kGated, kCols>(p, s);
-}
 
 template <class T, int kTokens>
 int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* flag, Scratch* scratch, cudaStream_t s) {
@@ -558,7 +542,11 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     if (a.tokens <= 32) return glu_few_launch<T, 32>(a, x, wg, wu, p.flag, &scratch, s);
     if (a.tokens <= 64) return glu_few_launch<T, 64>(a, x, wg, wu, p.flag, &scratch, s);
     if (a.tokens <= 128) return glu_few_launch<T, 128>(a, x, wg, wu, p.flag, &scratch, s);
-    return glu_forward<T, 256>(a, x, wg, wu, p, s);
+    ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kHalf));
+    ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
+    ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
+    p.row_tiles = div_up(a.tokens, kTile), p.col_tiles = div_up(a.hidden, kHalf);
+    return product_launch<T, kGated>(p, s);
 }
 
 template <class T>
@@ -585,14 +573,14 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         Operand wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
         ZKB_TRY(align<T>(&wg, a.in, F, &scratch, s));
         ZKB_TRY(align<T>(&wu, a.in, F, &scratch, s));
-        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, dg, a.tokens, F, ld, kRows));
-        ZKB_TRY(tc::make_map(&p.a[1], kCode<T>, du, a.tokens, F, ld, kRows));
-        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, F, wg.ld, 256));
-        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, F, wu.ld, 256));
+        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.a[1], kCode<T>, du, a.tokens, F, ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, F, wg.ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, F, wu.ld, kHalf));
         p.m = (unsigned)a.tokens, p.n = (unsigned)a.in, p.slices = div_up(F, kDepth);
-        p.row_tiles = div_up(p.m, kRows), p.col_tiles = div_up(p.n, 256);
+        p.row_tiles = div_up(p.m, kTile), p.col_tiles = div_up(p.n, kTile);
         p.out[0] = a.dx, p.ld[0] = a.lddx, p.wide[0] = copyable(a.dx, a.lddx);
-        ZKB_TRY((product_launch<T, kSummed, 256>(p, s)));
+        ZKB_TRY((product_launch<T, kSummed>(p, s)));
     }
     if (a.dwg) {
         Operand x = {a.x, a.ldx};
@@ -601,10 +589,10 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
         ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, du, a.tokens, F, ld, kDepth));
         p.m = (unsigned)a.in, p.n = (unsigned)F, p.slices = div_up(a.tokens, kDepth);
-        p.row_tiles = div_up(p.m, kRows), p.col_tiles = div_up(p.n, 256);
+        p.row_tiles = div_up(p.m, kTile), p.col_tiles = div_up(p.n, kTile);
         p.out[0] = a.dwg, p.ld[0] = a.lddwg, p.wide[0] = copyable(a.dwg, a.lddwg);
         p.out[1] = a.dwu, p.ld[1] = a.lddwu, p.wide[1] = copyable(a.dwu, a.lddwu);
-        ZKB_TRY((product_launch<T, kPaired, 256>(p, s)));
+        ZKB_TRY((product_launch<T, kPaired>(p, s)));
     }
     return ZKB_OK;
 }

@@ -57,10 +57,34 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, cons
     *reinterpret_cast<volatile int*>(w.flag) = 1;
     return false;
 }
+// some milliseconds: long after the copies and products that a block has in flight
+__device__ __forceinline__ void pause() {
+    const unsigned long long start = now_ns();
+    for (unsigned i = 0; i < (1u << 20) && now_ns() - start < 10000000ull; ++i) __nanosleep(1000);
+}
 // The flag that the kernels of this process raise (device and host address the same memory); null and the error text on failure.
 int* wait_flag();
 // Ends a call with an error if a wait of an earlier one ran out.
 int check_wait_flag(const char* who);
+
+// ---- clusters --------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// the same place in the shared memory of another block of the cluster
+__device__ __forceinline__ uint32_t address_in(uint32_t address, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(address), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void barrier_arrive_in(uint32_t cluster_address) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+}
 
 // ---- tensor copies ---------------------------------------------------------------------------------------------------------
 // [rows, cols] of 16-bit values, rows `ld` values apart, read in boxes of 64 columns (128 bytes, swizzled by 128) and box_rows rows;
@@ -77,6 +101,13 @@ __device__ __forceinline__ void load_box(const CUtensorMap* m, uint32_t dst, uin
         : "memory");
 }
 
+// The same copy by one block of a pair, arriving at a barrier of either (an address of the cluster's shared memory).
+__device__ __forceinline__ void load_box_pair(const CUtensorMap* m, uint32_t dst, uint32_t bar, int col, int row) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m),
+        "r"(bar), "r"(col), "r"(row)
+        : "memory");
+}
 // `bytes` consecutive bytes; both addresses and the size are multiples of 16
 __device__ __forceinline__ void load_bytes(uint32_t dst, unsigned long long src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
@@ -91,11 +122,22 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
 }
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t at, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t tmem, uint32_t cols) {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+}
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // arrives at the barrier when the products issued so far by this thread are done
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// the same for products of a pair, at the barriers of this place in both blocks
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 // A tile in shared memory, swizzled by 128 bytes.  K-major: rows of 128 bytes (64 values of k), groups of 8 rows 1024 bytes apart.  MN-major: k
 // rows of 128 bytes (64 values of m or n), groups of 8 k's 1024 bytes apart, groups of 64 m's or n's `group` bytes apart.
@@ -110,6 +152,13 @@ template <class T> __host__ __device__ constexpr uint32_t instruction(unsigned m
 __device__ __forceinline__ void product(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem), "l"(a), "l"(b),
+        "r"(instr), "r"((uint32_t)add)
+        : "memory");
+}
+// one product over both blocks of a pair, issued by the first: each block holds half of the rows of a and of d and half of the columns of b
+__device__ __forceinline__ void product_pair(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem), "l"(a), "l"(b),
         "r"(instr), "r"((uint32_t)add)
         : "memory");
 }
