@@ -8,28 +8,58 @@
 namespace zkb {
 namespace {
 
-// act(g) and, for the gradient, its derivative
-template <bool kDerivative>
-__device__ __forceinline__ float activate(int kind, float g, float* d) {
-    if (kind == ZKB_ACT_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-g));
+// act(g) and, for the gradient, its derivative.  1 / (1 + exp) by the approximate quotient (2^-22), which is far below a 16-bit step.
+template <int kAct, bool kDerivative>
+__device__ __forceinline__ float activate(float g, float* d) {
+    if constexpr (kAct == ZKB_ACT_SILU) {
+        const float s = __fdividef(1.0f, 1.0f + __expf(-g));
         if (kDerivative) *d = s * (1.0f + g * (1.0f - s));
         return g * s;
-    }
-    if (kind == ZKB_ACT_GELU) {
+    } else if constexpr (kAct == ZKB_ACT_GELU) {
         const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         if (kDerivative) *d = c + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
         return g * c;
-    }
-    if (kind == ZKB_ACT_GELU_TANH) {
+    } else if constexpr (kAct == ZKB_ACT_GELU_TANH) {
         // (1 + tanh k) / 2 = 1 / (1 + exp(-2k))
         const float k = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-        const float s = 1.0f / (1.0f + __expf(-2.0f * k));
+        const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * k));
         if (kDerivative) *d = s + 2.0f * g * s * (1.0f - s) * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
         return g * s;
+    } else {
+        if (kDerivative) *d = g > 0.0f ? 1.0f : 0.0f;
+        return g > 0.0f ? g : g != g ? g : 0.0f;
     }
-    if (kDerivative) *d = g > 0.0f ? 1.0f : 0.0f;
-    return fmaxf(g, 0.0f);
+}
+// h = act(g) * u in place of g
+template <int kAct, int N>
+__device__ __forceinline__ void gate_by(float (&g)[N], const float (&u)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = activate<kAct, false>(g[i], nullptr) * u[i];
+}
+template <int N>
+__device__ __forceinline__ void gate(int act, float (&g)[N], const float (&u)[N]) {
+    if (act == ZKB_ACT_SILU) gate_by<ZKB_ACT_SILU>(g, u);
+    else if (act == ZKB_ACT_GELU) gate_by<ZKB_ACT_GELU>(g, u);
+    else if (act == ZKB_ACT_GELU_TANH) gate_by<ZKB_ACT_GELU_TANH>(g, u);
+    else gate_by<ZKB_ACT_RELU>(g, u);
+}
+// the gradients of g and u, in their places, from that of h
+template <int kAct, int N>
+__device__ __forceinline__ void ungate_by(float (&g)[N], float (&u)[N], const float (&dh)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float da;
+        const float a = activate<kAct, true>(g[i], &da);
+        g[i] = dh[i] * u[i] * da;
+        u[i] = dh[i] * a;
+    }
+}
+template <int N>
+__device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], const float (&dh)[N]) {
+    if (act == ZKB_ACT_SILU) ungate_by<ZKB_ACT_SILU>(g, u, dh);
+    else if (act == ZKB_ACT_GELU) ungate_by<ZKB_ACT_GELU>(g, u, dh);
+    else if (act == ZKB_ACT_GELU_TANH) ungate_by<ZKB_ACT_GELU_TANH>(g, u, dh);
+    else ungate_by<ZKB_ACT_RELU>(g, u, dh);
 }
 
 // ---- the product kernel -----------------------------------------------------------------------------------------------------
@@ -39,27 +69,41 @@ __device__ __forceinline__ float activate(int kind, float g, float* d) {
 // blocks on their own would need 96.  In each block warp 0 copies 64-deep slices into a ring; in the first, warp 1 issues
 // the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 7 of both take their 128 rows of the other
 // accumulator out, so that a tile's epilogue runs beside the next tile's products.
-enum Form {
-    kGated,    // A x; B the two weights side by side, 128 columns of each in a tile; result act(g) * u
-    kSummed,   // A dg then du; B w_gate then w_up: one sum over both; result dx
-    kPaired    // A x^T; B dg for the first half of the tiles, du for the second; results dw_gate and dw_up
-};
+//
+// The forms of a tile:
+//   gated    first operand x; second the two weights side by side, 128 columns of each in a tile; result act(g) * u
+//   summed   dg, then du; w_gate, then w_up: one sum over both; result dx
+//   paired   x^T; dg for the first half of the tiles, du for the second; results dw_gate and dw_up
+// The gradients' launch holds tiles of both of the last: the few, long tiles of dx first, one or two to a pair of blocks, and the
+// many short ones of the weights where there is room.  The pairs with one tile of dx less take `head` of the short ones each before
+// the rest are dealt out to all, so that all end together.
 constexpr int kTile = 256, kHalf = 128, kDepth = 64;
 constexpr int kProductThreads = 256;
 constexpr int kStageBytes = 32 * 80;   // an epilogue warp's 32 x 32 values on their way out, rows 80 bytes apart
 constexpr int kRing = 6, kSlice = 2 * kHalf * kDepth * 2;
 constexpr size_t kProductSmem = 1024 + (size_t)kRing * kSlice + 4 * kStageBytes + 256;
 
-struct ProductArgs {
-    CUtensorMap a[2], b[2];
-    unsigned m, n;               // of the result (kGated: hidden)
-    unsigned row_tiles, col_tiles, slices;   // tiles of a result, slices of 64 of one sum
-    void* out[3];                // kGated: h, gate, up (or null); kSummed: dx; kPaired: dw_gate, dw_up
+struct Results {
+    unsigned m, n;                           // of one result (gated: hidden)
+    unsigned row_tiles, col_tiles, slices;   // its tiles, and slices of 64 of one sum
+    void* out[3];                            // gated: h, gate, up (or null); summed: dx; paired: dw_gate, dw_up
     size_t ld[3];
-    bool wide[3];                // 16-byte stores
+    bool wide[3];                            // 16-byte stores
+};
+struct GatedArgs {
+    CUtensorMap a, b[2];
+    Results r;
     int act;
     int* flag;
 };
+struct GradArgs {
+    CUtensorMap dg_rows[2], w[2];            // summed: dg and du in boxes of 128 rows, the weights
+    CUtensorMap x, dg_cols[2];               // paired: x, dg and du in boxes of 64 rows
+    Results dx, dw;
+    unsigned head;
+    int* flag;
+};
+struct Tile { unsigned row, col, pair; bool paired; };
 
 // 32 x 32 values of a warp (row i with lane i) to rows row0.. and columns col0.. of a matrix of m x n.
 template <class T>
@@ -88,8 +132,11 @@ __device__ __forceinline__ void store_block(char* stage, const float (&v)[32], T
             }
         }
     } else {
-        for (unsigned r = 0; r < 32 && row0 + r < m; ++r)
-            if (col0 + lane < n) out[(size_t)(row0 + r) * ld + col0 + lane] = *reinterpret_cast<const T*>(stage + r * 80 + lane * 2);
+        T* to = out + (size_t)row0 * ld + col0 + lane;
+        const unsigned rows = col0 + lane < n && row0 < m ? min(32u, m - row0) : 0;
+#pragma unroll 8
+        for (unsigned r = 0; r < 32; ++r)
+            if (r < rows) to[r * ld] = *reinterpret_cast<const T*>(stage + r * 80 + lane * 2);
     }
     __syncwarp();
 }
@@ -103,12 +150,38 @@ __device__ __forceinline__ void tile_place(unsigned tile, unsigned row_tiles, un
     *col = in / height;
 }
 
-template <class T, int kForm>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu_product_kernel(const __grid_constant__ ProductArgs p) {
-    constexpr bool kAMn = kForm == kPaired, kBMn = kForm != kSummed;
+// The i-th tile of a pair of blocks; false behind its last.
+__device__ __forceinline__ const Results& results_of(const GatedArgs& p, const Tile&) { return p.r; }
+__device__ __forceinline__ const Results& results_of(const GradArgs& p, const Tile& t) { return t.paired ? p.dw : p.dx; }
+__device__ __forceinline__ bool tile_of(const GatedArgs& p, unsigned i, unsigned me, unsigned pairs, Tile* t) {
+    const unsigned n = me + i * pairs;
+    if (n >= p.r.row_tiles * p.r.col_tiles) return false;
+    t->pair = 0, t->paired = false;
+    tile_place(n, p.r.row_tiles, p.r.col_tiles, &t->row, &t->col);
+    return true;
+}
+__device__ __forceinline__ bool tile_of(const GradArgs& p, unsigned i, unsigned me, unsigned pairs, Tile* t) {
+    const unsigned longs = p.dx.row_tiles * p.dx.col_tiles, more = longs % pairs, mine = longs / pairs + (me < more), per = p.dw.row_tiles * p.dw.col_tiles;
+    t->pair = 0, t->paired = i >= mine;
+    if (!t->paired) {
+        tile_place(me + i * pairs, p.dx.row_tiles, p.dx.col_tiles, &t->row, &t->col);
+        return true;
+    }
+    i -= mine;
+    unsigned n;
+    const unsigned ahead = more ? p.head : 0;
+    if (me >= more && i < ahead) n = me - more + i * (pairs - more);
+    else n = ahead * (pairs - more) + me + (i - (me >= more ? ahead : 0)) * pairs;
+    if (n >= 2 * per) return false;
+    t->pair = n / per;
+    tile_place(n % per, p.dw.row_tiles, p.dw.col_tiles, &t->row, &t->col);
+    return true;
+}
+
+template <class T, class Args>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu_product_kernel(const __grid_constant__ Args p) {
+    constexpr bool kGated = std::is_same<Args, GatedArgs>::value;
     constexpr int kA = kHalf * kDepth * 2;
-    constexpr uint32_t kInstruction = tc::instruction<T>(kTile, kTile, kAMn, kBMn);
-    constexpr int kSums = kForm == kSummed ? 2 : 1;
     extern __shared__ char raw[];
     char* ring = raw + ((1024 - (tc::smem_address(raw) & 1023)) & 1023);
     char* stages = ring + kRing * kSlice;
@@ -130,8 +203,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc::prefetch_map(&p.a[0]);
-        tc::prefetch_map(&p.b[0]);
     }
     if (warp == 2) tc::tmem_alloc_pair(tmem_at, 2 * kTile);
     tc::fence_before_sync();
@@ -142,56 +213,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
     grid_release();
     grid_wait();
 
-    const unsigned tiles = p.row_tiles * p.col_tiles, all = kForm == kPaired ? 2 * tiles : tiles;
-    const unsigned slices = p.slices * kSums, first = blockIdx.x / 2, step = gridDim.x / 2;
+    const unsigned first = blockIdx.x / 2, step = gridDim.x / 2;
     if (warp == 0 && lane == 0) {
         unsigned at = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (unsigned t = first; t < all && fine; t += step) {
-            unsigned row, col;
-            tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
-            const unsigned pair = t / tiles;
-            for (unsigned s = 0; s < slices; ++s) {
-                if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
-                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = tc::address_in(full + 8 * at, 0);
-                if (rank == 0) tc::barrier_expect(full + 8 * at, 2 * kSlice);
-                const int sum = kForm == kSummed ? (int)(s / p.slices) : 0;
-                const int k = (int)(s - sum * p.slices) * kDepth, m = row * kTile + rank * kHalf, n = col * kTile + rank * kHalf;
-                if constexpr (kAMn) {
-                    tc::load_box_pair(&p.a[0], a, bar, m, k);
-                    tc::load_box_pair(&p.a[0], a + 8192, bar, m + 64, k);
-                } else {
-                    tc::load_box_pair(&p.a[sum], a, bar, k, m);
+        Tile t;
+        for (unsigned i = 0; fine && tile_of(p, i, first, step, &t); ++i) {
+            const unsigned m = t.row * kTile + rank * kHalf, n = t.col * kTile + rank * kHalf;
+            const Results& r = results_of(p, t);
+            const unsigned sums = kGated || t.paired ? 1 : 2;
+            for (unsigned sum = 0; sum < sums && fine; ++sum)
+                for (unsigned s = 0; s < r.slices; ++s) {
+                    if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
+                    const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = tc::address_in(full + 8 * at, 0);
+                    if (rank == 0) tc::barrier_expect(full + 8 * at, 2 * kSlice);
+                    const int k = s * kDepth;
+                    if constexpr (kGated) {   // the first block holds w_gate's columns, the second w_up's
+                        tc::load_box_pair(&p.a, a, bar, k, m);
+                        tc::load_box_pair(&p.b[rank], b, bar, t.col * kHalf, k);
+                        tc::load_box_pair(&p.b[rank], b + 8192, bar, t.col * kHalf + 64, k);
+                    } else if (t.paired) {
+                        tc::load_box_pair(&p.x, a, bar, m, k);
+                        tc::load_box_pair(&p.x, a + 8192, bar, m + 64, k);
+                        tc::load_box_pair(&p.dg_cols[t.pair], b, bar, n, k);
+                        tc::load_box_pair(&p.dg_cols[t.pair], b + 8192, bar, n + 64, k);
+                    } else {
+                        tc::load_box_pair(&p.dg_rows[sum], a, bar, k, m);
+                        tc::load_box_pair(&p.w[sum], b, bar, k, n);
+                    }
+                    if (++at == kRing) { at = 0; phase ^= 1; }
                 }
-                if constexpr (kForm == kGated) {   // the first block holds w_gate's columns, the second w_up's
-                    tc::load_box_pair(&p.b[rank], b, bar, col * kHalf, k);
-                    tc::load_box_pair(&p.b[rank], b + 8192, bar, col * kHalf + 64, k);
-                } else if constexpr (kForm == kPaired) {
-                    tc::load_box_pair(&p.b[pair], b, bar, n, k);
-                    tc::load_box_pair(&p.b[pair], b + 8192, bar, n + 64, k);
-                } else {
-                    tc::load_box_pair(&p.b[sum], b, bar, k, n);
-                }
-                if (++at == kRing) { at = 0; phase ^= 1; }
-            }
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
-        unsigned at = 0, count = 0;
+        unsigned at = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (unsigned t = first; t < all && fine; t += step, ++count) {
-            const unsigned acc = count & 1;
-            if (!tc::barrier_wait(taken + 8 * acc, ((count >> 1) & 1) ^ 1, watch)) break;
+        Tile t;
+        for (unsigned i = 0; fine && tile_of(p, i, first, step, &t); ++i) {
+            const unsigned acc = i & 1;
+            if (!tc::barrier_wait(taken + 8 * acc, ((i >> 1) & 1) ^ 1, watch)) break;
             tc::fence_after_sync();
+            const bool a_mn = !kGated && t.paired, b_mn = kGated || t.paired;
+            const uint32_t instruction = tc::instruction<T>(kTile, kTile, a_mn, b_mn), a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+            const unsigned slices = results_of(p, t).slices * (kGated || t.paired ? 1 : 2);
             for (unsigned s = 0; s < slices; ++s) {
                 if (!tc::barrier_wait(full + 8 * at, phase, watch)) { fine = false; break; }
                 tc::fence_after_sync();
                 const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA;
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; ++k)
-                    tc::product_pair(tmem + acc * kTile, tc::tile_descriptor(a + k * (kAMn ? 2048 : 32), kAMn, 8192),
-                                     tc::tile_descriptor(b + k * (kBMn ? 2048 : 32), kBMn, 8192), kInstruction, s || k);
+                    tc::product_pair(tmem + acc * kTile, tc::tile_descriptor(a + k * a_step, a_mn, 8192), tc::tile_descriptor(b + k * b_step, b_mn, 8192),
+                                     instruction, s || k);
                 tc::commit_pair(empty + 8 * at);
                 if (++at == kRing) { at = 0; phase ^= 1; }
             }
@@ -199,35 +272,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         }
     } else if (warp >= 4) {
         char* stage = stages + (warp - 4) * kStageBytes;
-        unsigned count = 0;
-        for (unsigned t = first; t < all; t += step, ++count) {
-            unsigned row, col;
-            tile_place(t % tiles, p.row_tiles, p.col_tiles, &row, &col);
-            const unsigned acc = count & 1, pair = t / tiles;
-            const bool fine = tc::barrier_wait(ready + 8 * acc, (count >> 1) & 1, watch);
+        Tile t;
+        for (unsigned i = 0; tile_of(p, i, first, step, &t); ++i) {
+            const unsigned acc = i & 1;
+            const bool fine = tc::barrier_wait(ready + 8 * acc, (i >> 1) & 1, watch);
             if (!__all_sync(0xffffffffu, fine)) break;
             tc::fence_after_sync();
             const uint32_t from = tmem + ((warp - 4) * 32 << 16) + acc * kTile;
-            const unsigned row0 = row * kTile + rank * kHalf + (warp - 4) * 32;
-            if constexpr (kForm == kGated) {
+            const unsigned row0 = t.row * kTile + rank * kHalf + (warp - 4) * 32;
+            const Results& r = results_of(p, t);
+            if constexpr (kGated) {
                 for (int c = 0; c < kHalf; c += 32) {
                     float g[32], u[32];
                     tc::load_columns(from + c, g);
                     tc::load_columns(from + kHalf + c, u);
-                    const unsigned col0 = col * kHalf + c;
-                    if (p.out[1]) {
-                        store_block<T>(stage, g, static_cast<T*>(p.out[1]), p.ld[1], p.wide[1], row0, col0, p.m, p.n);
-                        store_block<T>(stage, u, static_cast<T*>(p.out[2]), p.ld[2], p.wide[2], row0, col0, p.m, p.n);
+                    const unsigned col0 = t.col * kHalf + c;
+                    if (r.out[1]) {
+                        store_block<T>(stage, g, static_cast<T*>(r.out[1]), r.ld[1], r.wide[1], row0, col0, r.m, r.n);
+                        store_block<T>(stage, u, static_cast<T*>(r.out[2]), r.ld[2], r.wide[2], row0, col0, r.m, r.n);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) g[i] = activate<false>(p.act, g[i], nullptr) * u[i];
-                    store_block<T>(stage, g, static_cast<T*>(p.out[0]), p.ld[0], p.wide[0], row0, col0, p.m, p.n);
+                    gate(p.act, g, u);
+                    store_block<T>(stage, g, static_cast<T*>(r.out[0]), r.ld[0], r.wide[0], row0, col0, r.m, r.n);
                 }
             } else {
                 for (int c = 0; c < kTile; c += 32) {
                     float v[32];
                     tc::load_columns(from + c, v);
-                    store_block<T>(stage, v, static_cast<T*>(p.out[pair]), p.ld[pair], p.wide[pair], row0, col * kTile + c, p.m, p.n);
+                    store_block<T>(stage, v, static_cast<T*>(r.out[t.pair]), r.ld[t.pair], r.wide[t.pair], row0, t.col * kTile + c, r.m, r.n);
                 }
             }
             tc::fence_before_sync();
@@ -408,7 +479,9 @@ __global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_c
         static_cast<T*>(p.out[1])[t * p.ld[1] + f] = from_f32<T>(g);
         static_cast<T*>(p.out[2])[t * p.ld[2] + f] = from_f32<T>(u);
     }
-    static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(activate<false>(p.act, g, nullptr) * u);
+    float h[1] = {g};
+    gate(p.act, h, {u});
+    static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(h[0]);
 }
 
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
@@ -436,13 +509,7 @@ __global__ void __launch_bounds__(256) glu_split_kernel(const T* __restrict__ ga
                 d[j] = in ? to_f32<T>(dh[m * ldh + n + j]) : 0.0f;
             }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float da;
-            const float a = activate<true>(act, g[j], &da);
-            g[j] = d[j] * u[j] * da;
-            u[j] = d[j] * a;
-        }
+        ungate(act, g, u, d);
         store_vec<T, 8>(dg + m * ld + n, g);
         store_vec<T, 8>(du + m * ld + n, u);
     }
@@ -489,13 +556,17 @@ int align(Operand* x, size_t rows, size_t cols, Scratch* scratch, cudaStream_t s
     return ZKB_OK;
 }
 
-template <class T, int kForm>
-int product_launch(const ProductArgs& p, cudaStream_t s) {
-    const auto glu_product = glu_product_kernel<T, kForm>;
+template <class T, class Args>
+int product_launch(const Args& p, size_t tiles, cudaStream_t s) {
+    const auto glu_product = glu_product_kernel<T, Args>;
     ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kProductSmem));
-    const unsigned tiles = p.row_tiles * p.col_tiles * (kForm == kPaired ? 2 : 1);
-    return launch_beside("glu_product", glu_product, 2 * std::min(tiles, (unsigned)sm_count() / 2), kProductThreads, kProductSmem, s, p);
+    return launch_beside("glu_product", glu_product, 2 * (unsigned)std::min(tiles, (size_t)sm_count() / 2), kProductThreads, kProductSmem, s, p);
 }
+void lay_results(Results* r, size_t m, size_t n, unsigned tile_cols, size_t k) {
+    r->m = (unsigned)m, r->n = (unsigned)n, r->slices = div_up(k, kDepth);
+    r->row_tiles = div_up(m, kTile), r->col_tiles = div_up(n, tile_cols);
+}
+void set_result(Results* r, int i, void* out, size_t ld) { r->out[i] = out, r->ld[i] = ld, r->wide[i] = copyable(out, ld); }
 
 template <class T> constexpr int kCode = std::is_same<T, __half>::value ? ZKB_F16 : ZKB_BF16;
 
@@ -530,23 +601,22 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
     ZKB_TRY(align<T>(&wg, a.in, a.hidden, &scratch, s));
     ZKB_TRY(align<T>(&wu, a.in, a.hidden, &scratch, s));
-    ProductArgs p = {};
-    p.m = (unsigned)a.tokens, p.n = (unsigned)a.hidden, p.slices = div_up(a.in, kDepth);
-    p.out[0] = a.h, p.out[1] = a.gate_out, p.out[2] = a.up_out;
-    p.ld[0] = a.ldh, p.ld[1] = a.ldg, p.ld[2] = a.ldu;
-    for (int i = 0; i < 3; ++i) p.wide[i] = copyable(p.out[i], p.ld[i]);
-    p.act = a.act;
-    p.flag = tc::wait_flag();
-    if (!p.flag) return ZKB_ERR_CUDA;
-    if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, p.flag, &scratch, s);
-    if (a.tokens <= 32) return glu_few_launch<T, 32>(a, x, wg, wu, p.flag, &scratch, s);
-    if (a.tokens <= 64) return glu_few_launch<T, 64>(a, x, wg, wu, p.flag, &scratch, s);
-    if (a.tokens <= 128) return glu_few_launch<T, 128>(a, x, wg, wu, p.flag, &scratch, s);
-    ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kHalf));
+    int* const flag = tc::wait_flag();
+    if (!flag) return ZKB_ERR_CUDA;
+    if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, flag, &scratch, s);
+    if (a.tokens <= 32) return glu_few_launch<T, 32>(a, x, wg, wu, flag, &scratch, s);
+    if (a.tokens <= 64) return glu_few_launch<T, 64>(a, x, wg, wu, flag, &scratch, s);
+    if (a.tokens <= 128) return glu_few_launch<T, 128>(a, x, wg, wu, flag, &scratch, s);
+    GatedArgs p = {};
+    p.act = a.act, p.flag = flag;
+    ZKB_TRY(tc::make_map(&p.a, kCode<T>, x.p, a.tokens, a.in, x.ld, kHalf));
     ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
     ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
-    p.row_tiles = div_up(a.tokens, kTile), p.col_tiles = div_up(a.hidden, kHalf);
-    return product_launch<T, kGated>(p, s);
+    lay_results(&p.r, a.tokens, a.hidden, kHalf, a.in);
+    set_result(&p.r, 0, a.h, a.ldh);
+    set_result(&p.r, 1, a.gate_out, a.ldg);
+    set_result(&p.r, 2, a.up_out, a.ldu);
+    return product_launch<T>(p, (size_t)p.r.row_tiles * p.r.col_tiles, s);
 }
 
 template <class T>
@@ -566,35 +636,33 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, 8> : glu_split_kernel<T, 1>;
     ZKB_TRY(launch_beside("glu_split", glu_split, (unsigned)std::min<size_t>((a.tokens * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
                static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld, a.tokens, F, a.act));
-    ProductArgs p = {};
-    p.flag = tc::wait_flag();
-    if (!p.flag) return ZKB_ERR_CUDA;
+    GradArgs p = {};
+    if (!(p.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
     if (a.dx) {
         Operand wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
         ZKB_TRY(align<T>(&wg, a.in, F, &scratch, s));
         ZKB_TRY(align<T>(&wu, a.in, F, &scratch, s));
-        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
-        ZKB_TRY(tc::make_map(&p.a[1], kCode<T>, du, a.tokens, F, ld, kHalf));
-        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, F, wg.ld, kHalf));
-        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, F, wu.ld, kHalf));
-        p.m = (unsigned)a.tokens, p.n = (unsigned)a.in, p.slices = div_up(F, kDepth);
-        p.row_tiles = div_up(p.m, kTile), p.col_tiles = div_up(p.n, kTile);
-        p.out[0] = a.dx, p.ld[0] = a.lddx, p.wide[0] = copyable(a.dx, a.lddx);
-        ZKB_TRY((product_launch<T, kSummed>(p, s)));
+        ZKB_TRY(tc::make_map(&p.dg_rows[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.dg_rows[1], kCode<T>, du, a.tokens, F, ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.w[0], kCode<T>, wg.p, a.in, F, wg.ld, kHalf));
+        ZKB_TRY(tc::make_map(&p.w[1], kCode<T>, wu.p, a.in, F, wu.ld, kHalf));
+        lay_results(&p.dx, a.tokens, a.in, kTile, F);
+        set_result(&p.dx, 0, a.dx, a.lddx);
     }
     if (a.dwg) {
         Operand x = {a.x, a.ldx};
         ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
-        ZKB_TRY(tc::make_map(&p.a[0], kCode<T>, x.p, a.tokens, a.in, x.ld, kDepth));
-        ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
-        ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, du, a.tokens, F, ld, kDepth));
-        p.m = (unsigned)a.in, p.n = (unsigned)F, p.slices = div_up(a.tokens, kDepth);
-        p.row_tiles = div_up(p.m, kTile), p.col_tiles = div_up(p.n, kTile);
-        p.out[0] = a.dwg, p.ld[0] = a.lddwg, p.wide[0] = copyable(a.dwg, a.lddwg);
-        p.out[1] = a.dwu, p.ld[1] = a.lddwu, p.wide[1] = copyable(a.dwu, a.lddwu);
-        ZKB_TRY((product_launch<T, kPaired>(p, s)));
+        ZKB_TRY(tc::make_map(&p.x, kCode<T>, x.p, a.tokens, a.in, x.ld, kDepth));
+        ZKB_TRY(tc::make_map(&p.dg_cols[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
+        ZKB_TRY(tc::make_map(&p.dg_cols[1], kCode<T>, du, a.tokens, F, ld, kDepth));
+        lay_results(&p.dw, a.in, F, kTile, a.tokens);
+        set_result(&p.dw, 0, a.dwg, a.lddwg);
+        set_result(&p.dw, 1, a.dwu, a.lddwu);
     }
-    return ZKB_OK;
+    const size_t longs = (size_t)p.dx.row_tiles * p.dx.col_tiles, shorts = 2 * (size_t)p.dw.row_tiles * p.dw.col_tiles;
+    const size_t pairs = std::min(longs + shorts, (size_t)sm_count() / 2), spare = pairs - longs % pairs;
+    if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((2 * p.dx.slices + p.dw.slices / 2) / p.dw.slices, shorts / spare);
+    return product_launch<T>(p, longs + shorts, s);
 }
 
 int check_matrix(const char* who, const char* name, const void* p, size_t rows, size_t cols, size_t ld, bool needed) {
