@@ -2,6 +2,8 @@
 //
 // Weights are [in, hidden], as zkFC and FrTensor::matmul take them.  Sums are in 32 bits; h is formed from the unrounded sums.
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include "tensorcore.cuh"
 
@@ -76,12 +78,14 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 //   paired   x^T; dg for the first half of the tiles, du for the second; results dw_gate and dw_up
 // The gradients' launch holds tiles of both of the last: the few, long tiles of dx first, one or two to a pair of blocks, and the
 // many short ones of the weights where there is room.  The pairs with one tile of dx less take `head` of the short ones each before
-// the rest are dealt out to all, so that all end together.
+// the rest are dealt out to all, so that all end together.  Where dx has fewer tiles than there are pairs, each of its sums is cut
+// into parts, which are left in 32 bits and added in order by glu_add_parts_kernel.
 constexpr int kTile = 256, kHalf = 128, kDepth = 64;
-constexpr int kProductThreads = 256;
+constexpr int kTakers = 4;             // epilogue warps of a block (8 were no faster)
+constexpr int kProductThreads = 128 + 32 * kTakers;
 constexpr int kStageBytes = 32 * 80;   // an epilogue warp's 32 x 32 values on their way out, rows 80 bytes apart
 constexpr int kRing = 6, kSlice = 2 * kHalf * kDepth * 2;
-constexpr size_t kProductSmem = 1024 + (size_t)kRing * kSlice + 4 * kStageBytes + 256;
+constexpr size_t kProductSmem = 1024 + (size_t)kRing * kSlice + kTakers * kStageBytes + 256;
 
 struct Results {
     unsigned m, n;                           // of one result (gated: hidden)
@@ -100,10 +104,12 @@ struct GradArgs {
     CUtensorMap dg_rows[2], w[2];            // summed: dg and du in boxes of 128 rows, the weights
     CUtensorMap x, dg_cols[2];               // paired: x, dg and du in boxes of 64 rows
     Results dx, dw;
-    unsigned head;
+    unsigned head, parts;                    // parts: of dx's sums
+    float* sums;                             // [parts][m][sums_ld], if there are several
+    unsigned sums_ld;
     int* flag;
 };
-struct Tile { unsigned row, col, pair; bool paired; };
+struct Tile { unsigned row, col, pair, part, from, to; bool paired; };   // from, to: its slices
 
 // 32 x 32 values of a warp (row i with lane i) to rows row0.. and columns col0.. of a matrix of m x n.
 template <class T>
@@ -156,15 +162,19 @@ __device__ __forceinline__ const Results& results_of(const GradArgs& p, const Ti
 __device__ __forceinline__ bool tile_of(const GatedArgs& p, unsigned i, unsigned me, unsigned pairs, Tile* t) {
     const unsigned n = me + i * pairs;
     if (n >= p.r.row_tiles * p.r.col_tiles) return false;
-    t->pair = 0, t->paired = false;
+    t->pair = t->part = t->from = 0, t->to = p.r.slices, t->paired = false;
     tile_place(n, p.r.row_tiles, p.r.col_tiles, &t->row, &t->col);
     return true;
 }
 __device__ __forceinline__ bool tile_of(const GradArgs& p, unsigned i, unsigned me, unsigned pairs, Tile* t) {
-    const unsigned longs = p.dx.row_tiles * p.dx.col_tiles, more = longs % pairs, mine = longs / pairs + (me < more), per = p.dw.row_tiles * p.dw.col_tiles;
-    t->pair = 0, t->paired = i >= mine;
+    const unsigned whole = p.dx.row_tiles * p.dx.col_tiles, longs = whole * p.parts, more = longs % pairs, mine = longs / pairs + (me < more);
+    const unsigned per = p.dw.row_tiles * p.dw.col_tiles;
+    t->pair = t->part = 0, t->paired = i >= mine;
     if (!t->paired) {
-        tile_place(me + i * pairs, p.dx.row_tiles, p.dx.col_tiles, &t->row, &t->col);
+        const unsigned n = me + i * pairs;
+        t->part = n / whole;
+        t->from = 2 * p.dx.slices * t->part / p.parts, t->to = 2 * p.dx.slices * (t->part + 1) / p.parts;
+        tile_place(n % whole, p.dx.row_tiles, p.dx.col_tiles, &t->row, &t->col);
         return true;
     }
     i -= mine;
@@ -174,6 +184,7 @@ __device__ __forceinline__ bool tile_of(const GradArgs& p, unsigned i, unsigned 
     else n = ahead * (pairs - more) + me + (i - (me >= more ? ahead : 0)) * pairs;
     if (n >= 2 * per) return false;
     t->pair = n / per;
+    t->from = 0, t->to = p.dw.slices;
     tile_place(n % per, p.dw.row_tiles, p.dw.col_tiles, &t->row, &t->col);
     return true;
 }
@@ -185,7 +196,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
     extern __shared__ char raw[];
     char* ring = raw + ((1024 - (tc::smem_address(raw) & 1023)) & 1023);
     char* stages = ring + kRing * kSlice;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(stages + 4 * kStageBytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stages + kTakers * kStageBytes);
     volatile int* dead = reinterpret_cast<volatile int*>(bars + 2 * kRing + 4);
     const uint32_t full = tc::smem_address(bars), empty = full + 8 * kRing, ready = empty + 8 * kRing, taken = ready + 16;
     const uint32_t tmem_at = taken + 24;
@@ -198,7 +209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         }
         for (int i = 0; i < 2; ++i) {
             tc::barrier_init(ready + 8 * i, 1);
-            tc::barrier_init(taken + 8 * i, 8);   // the epilogue warps of both blocks
+            tc::barrier_init(taken + 8 * i, 2 * kTakers);   // the epilogue warps of both blocks
         }
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -210,8 +221,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
     tc::cluster_barrier();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kRing + 5);
-    grid_release();
-    grid_wait();
 
     const unsigned first = blockIdx.x / 2, step = gridDim.x / 2;
     if (warp == 0 && lane == 0) {
@@ -222,28 +231,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         for (unsigned i = 0; fine && tile_of(p, i, first, step, &t); ++i) {
             const unsigned m = t.row * kTile + rank * kHalf, n = t.col * kTile + rank * kHalf;
             const Results& r = results_of(p, t);
-            const unsigned sums = kGated || t.paired ? 1 : 2;
-            for (unsigned sum = 0; sum < sums && fine; ++sum)
-                for (unsigned s = 0; s < r.slices; ++s) {
-                    if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
-                    const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = tc::address_in(full + 8 * at, 0);
-                    if (rank == 0) tc::barrier_expect(full + 8 * at, 2 * kSlice);
-                    const int k = s * kDepth;
-                    if constexpr (kGated) {   // the first block holds w_gate's columns, the second w_up's
-                        tc::load_box_pair(&p.a, a, bar, k, m);
-                        tc::load_box_pair(&p.b[rank], b, bar, t.col * kHalf, k);
-                        tc::load_box_pair(&p.b[rank], b + 8192, bar, t.col * kHalf + 64, k);
-                    } else if (t.paired) {
-                        tc::load_box_pair(&p.x, a, bar, m, k);
-                        tc::load_box_pair(&p.x, a + 8192, bar, m + 64, k);
-                        tc::load_box_pair(&p.dg_cols[t.pair], b, bar, n, k);
-                        tc::load_box_pair(&p.dg_cols[t.pair], b + 8192, bar, n + 64, k);
-                    } else {
-                        tc::load_box_pair(&p.dg_rows[sum], a, bar, k, m);
-                        tc::load_box_pair(&p.w[sum], b, bar, k, n);
-                    }
-                    if (++at == kRing) { at = 0; phase ^= 1; }
+            for (unsigned s = t.from; s < t.to; ++s) {
+                if (!tc::barrier_wait(empty + 8 * at, phase ^ 1, watch)) { fine = false; break; }
+                const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA, bar = tc::address_in(full + 8 * at, 0);
+                if (rank == 0) tc::barrier_expect(full + 8 * at, 2 * kSlice);
+                const unsigned sum = s >= r.slices;
+                const int k = (s - sum * r.slices) * kDepth;
+                if constexpr (kGated) {   // the first block holds w_gate's columns, the second w_up's
+                    tc::load_box_pair(&p.a, a, bar, k, m);
+                    tc::load_box_pair(&p.b[rank], b, bar, t.col * kHalf, k);
+                    tc::load_box_pair(&p.b[rank], b + 8192, bar, t.col * kHalf + 64, k);
+                } else if (t.paired) {
+                    tc::load_box_pair(&p.x, a, bar, m, k);
+                    tc::load_box_pair(&p.x, a + 8192, bar, m + 64, k);
+                    tc::load_box_pair(&p.dg_cols[t.pair], b, bar, n, k);
+                    tc::load_box_pair(&p.dg_cols[t.pair], b + 8192, bar, n + 64, k);
+                } else {
+                    tc::load_box_pair(&p.dg_rows[sum], a, bar, k, m);
+                    tc::load_box_pair(&p.w[sum], b, bar, k, n);
                 }
+                if (++at == kRing) { at = 0; phase ^= 1; }
+            }
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         unsigned at = 0;
@@ -256,15 +264,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
             tc::fence_after_sync();
             const bool a_mn = !kGated && t.paired, b_mn = kGated || t.paired;
             const uint32_t instruction = tc::instruction<T>(kTile, kTile, a_mn, b_mn), a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
-            const unsigned slices = results_of(p, t).slices * (kGated || t.paired ? 1 : 2);
-            for (unsigned s = 0; s < slices; ++s) {
+            for (unsigned s = t.from; s < t.to; ++s) {
                 if (!tc::barrier_wait(full + 8 * at, phase, watch)) { fine = false; break; }
                 tc::fence_after_sync();
                 const uint32_t a = tc::smem_address(ring) + at * kSlice, b = a + kA;
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; ++k)
                     tc::product_pair(tmem + acc * kTile, tc::tile_descriptor(a + k * a_step, a_mn, 8192), tc::tile_descriptor(b + k * b_step, b_mn, 8192),
-                                     instruction, s || k);
+                                     instruction, s > t.from || k);
                 tc::commit_pair(empty + 8 * at);
                 if (++at == kRing) { at = 0; phase ^= 1; }
             }
@@ -275,14 +282,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         Tile t;
         for (unsigned i = 0; tile_of(p, i, first, step, &t); ++i) {
             const unsigned acc = i & 1;
-            const bool fine = tc::barrier_wait(ready + 8 * acc, (i >> 1) & 1, watch);
-            if (!__all_sync(0xffffffffu, fine)) break;
+            if (!tc::barrier_wait_warp(ready + 8 * acc, (i >> 1) & 1, watch)) break;
             tc::fence_after_sync();
-            const uint32_t from = tmem + ((warp - 4) * 32 << 16) + acc * kTile;
-            const unsigned row0 = t.row * kTile + rank * kHalf + (warp - 4) * 32;
+            const uint32_t from = tmem + (warp % 4 * 32 << 16) + acc * kTile;
+            const unsigned row0 = t.row * kTile + rank * kHalf + warp % 4 * 32;
             const Results& r = results_of(p, t);
             if constexpr (kGated) {
-                for (int c = 0; c < kHalf; c += 32) {
+                for (unsigned c = 0; c < kHalf; c += 32) {
                     float g[32], u[32];
                     tc::load_columns(from + c, g);
                     tc::load_columns(from + kHalf + c, u);
@@ -295,10 +301,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
                     store_block<T>(stage, g, static_cast<T*>(r.out[0]), r.ld[0], r.wide[0], row0, col0, r.m, r.n);
                 }
             } else {
-                for (int c = 0; c < kTile; c += 32) {
+                for (unsigned c = 0; c < kTile; c += 32) {
                     float v[32];
                     tc::load_columns(from + c, v);
-                    store_block<T>(stage, v, static_cast<T*>(r.out[t.pair]), r.ld[t.pair], r.wide[t.pair], row0, t.col * kTile + c, r.m, r.n);
+                    const unsigned col0 = t.col * kTile + c;
+                    if (!t.paired && p.parts > 1) {   // this lane's row of a part, as it is
+                        float* to = p.sums + ((size_t)t.part * r.m + row0 + lane) * p.sums_ld + col0;
+                        if (row0 + lane < r.m)
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                if (col0 + j < p.sums_ld) *reinterpret_cast<float4*>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        __syncwarp();   // the next columns are read by the warp as one
+                        continue;
+                    }
+                    store_block<T>(stage, v, static_cast<T*>(r.out[t.pair]), r.ld[t.pair], r.wide[t.pair], row0, col0, r.m, r.n);
                 }
             }
             tc::fence_before_sync();
@@ -325,7 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
 // (part of a) tile in the workspace; glu_few_finish_kernel adds the parts of a tile, in order, and applies the activation.
 // Parts of a cluster that share a tile through distributed shared memory were measured before: no more than one such block ran on an
 // SM, and the ring of 72 KB that left to each read 4.0 TB/s.
-constexpr int kFewCols = 128;
+constexpr int kFewCols = 128, kFewThreads = 256;
 template <int kTokens> constexpr int kFewSlice = (2 * kFewCols + kTokens) * kDepth * 2;
 template <int kTokens> constexpr int kFewRing = kTokens <= 32 ? 6 : kTokens == 64 ? 5 : 4;
 template <int kTokens> constexpr size_t few_smem() { return 1024 + (size_t)kFewRing<kTokens> * kFewSlice<kTokens> + 256; }
@@ -353,7 +369,7 @@ __device__ __forceinline__ unsigned run_of(unsigned slice, unsigned blocks, unsi
 }
 
 template <class T, int kTokens>
-__global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_constant__ FewArgs p) {
+__global__ void __launch_bounds__(kFewThreads) glu_few_kernel(const __grid_constant__ FewArgs p) {
     constexpr int kA = kFewCols * kDepth * 2, kSlice = kFewSlice<kTokens>, kR = kFewRing<kTokens>;
     constexpr uint32_t kInstruction = tc::instruction<T>(kFewCols, kTokens, true, false);
     constexpr uint32_t kAcc = 2 * kTokens;
@@ -385,8 +401,6 @@ __global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_c
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
-    grid_release();
-    grid_wait();
 
     if (warp == 0 && lane == 0) {
         unsigned issued = 0;
@@ -432,8 +446,7 @@ __global__ void __launch_bounds__(kProductThreads) glu_few_kernel(const __grid_c
         unsigned count = 0;
         for (unsigned tile = first / p.slices; tile <= (last - 1) / p.slices; ++tile, ++count) {
             const unsigned acc = count & 1;
-            const bool fine = tc::barrier_wait(ready + 8 * acc, (count >> 1) & 1, watch);
-            if (!__all_sync(0xffffffffu, fine)) break;
+            if (!tc::barrier_wait_warp(ready + 8 * acc, (count >> 1) & 1, watch)) break;
             tc::fence_after_sync();
             float* to = p.parts + (size_t)(tile + blockIdx.x) * p.tokens * 2 * kFewCols + (warp - 4) * 32 + lane;
             for (unsigned t0 = 0; t0 < p.tokens; t0 += 16) {
@@ -484,34 +497,74 @@ __global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_c
     static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(h[0]);
 }
 
+// 8 values from any address, of which `count` (1 to 8) belong to the row; the others come back as they may.  Reads whole 16-byte
+// granules, the second only where it holds one of the row's values, so that nothing beyond the row's own pages is touched.
+template <class T>
+__device__ __forceinline__ Vec<T, 8> load_any(const T* p, unsigned count) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const unsigned off = at & 15;
+    const uint4* from = reinterpret_cast<const uint4*>(at - off);
+    const uint4 a = __ldg(from);
+    uint4 b = make_uint4(0, 0, 0, 0);
+    if (off + count * 2 > 16) b = __ldg(from + 1);
+    const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const unsigned word = off >> 2, bits = (off & 3) * 8;
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = word < 2 ? (word ? x[i + 1] : x[i]) : (word == 2 ? x[i + 2] : x[i + 3]);
+    union { uint32_t u[4]; Vec<T, 8> v; } out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.u[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    return out.v;
+}
+
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
 // follow have to be: each is off by half a step at most, independently, so a sum over them is off by no more, relative to its
 // norm, than its own rounding.
-template <class T, int V>
-__global__ void __launch_bounds__(256) glu_split_kernel(const T* __restrict__ gate, size_t ldg, const T* __restrict__ up, size_t ldu, const T* __restrict__ dh,
-                                                        size_t ldh, T* __restrict__ dg, T* __restrict__ du, size_t ld, size_t rows, size_t cols, int act) {
-    grid_release();
-    grid_wait();
-    const size_t vecs = ld / 8;
-    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
-        const size_t m = i / vecs, n = i % vecs * 8;
+template <class T, bool kWidePath>
+__global__ void __launch_bounds__(128) glu_split_kernel(const T* __restrict__ gate, size_t ldg, const T* __restrict__ up, size_t ldu, const T* __restrict__ dh,
+                                                        size_t ldh, T* __restrict__ dg, T* __restrict__ du, size_t ld, unsigned rows, unsigned cols, int act) {
+    const unsigned n = (blockIdx.x * 128 + threadIdx.x) * 8;
+    if (n >= cols) return;
+    for (unsigned m = blockIdx.y; m < rows; m += gridDim.y) {
         float g[8], u[8], d[8];
-        if (V == 8 && n + 8 <= cols) {
+        if (kWidePath && n + 8 <= cols) {
             load_vec<T, 8>(gate + m * ldg + n, g);
             load_vec<T, 8>(up + m * ldu + n, u);
             load_vec<T, 8>(dh + m * ldh + n, d);
         } else {
+            const unsigned count = min(8u, cols - n);
+            const Vec<T, 8> a = load_any<T>(gate + m * ldg + n, count), b = load_any<T>(up + m * ldu + n, count), c = load_any<T>(dh + m * ldh + n, count);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool in = n + j < cols;
-                g[j] = in ? to_f32<T>(gate[m * ldg + n + j]) : 0.0f;
-                u[j] = in ? to_f32<T>(up[m * ldu + n + j]) : 0.0f;
-                d[j] = in ? to_f32<T>(dh[m * ldh + n + j]) : 0.0f;
-            }
+            for (int j = 0; j < 8; ++j) g[j] = to_f32<T>(a.v[j]), u[j] = to_f32<T>(b.v[j]), d[j] = to_f32<T>(c.v[j]);
         }
         ungate(act, g, u, d);
         store_vec<T, 8>(dg + m * ld + n, g);
         store_vec<T, 8>(du + m * ld + n, u);
+    }
+}
+
+// dx from the parts of its sums, in their order
+template <class T, bool kWidePath>
+__global__ void __launch_bounds__(128) glu_add_parts_kernel(const float* __restrict__ sums, unsigned parts, unsigned m, unsigned n, unsigned ld, T* __restrict__ out,
+                                                            size_t ldo) {
+    grid_release();
+    grid_wait();
+    const unsigned c = (blockIdx.x * 128 + threadIdx.x) * 4, row = blockIdx.y;
+    if (c >= n) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (unsigned k = 0; k < parts; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(sums + ((size_t)k * m + row) * ld + c);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    T* to = out + (size_t)row * ldo + c;
+    if (kWidePath && c + 4 <= n) {
+        store_vec<T, 4>(to, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < n) to[j] = from_f32<T>(v[j]);
     }
 }
 
@@ -525,34 +578,44 @@ struct GluArgs {
 };
 
 // Rows that a tensor copy cannot read (an address or a stride that is no multiple of 16 bytes), laid out anew with a stride of
-// whole 16 bytes: one pass over the operand before the products.
+// whole 16 bytes: one pass over the operands before the products.
+struct Operand { const void* p; size_t ld, rows, cols; };
+struct AlignArgs {
+    Operand from[3];
+    void* to[3];
+    size_t ld_to[3];
+};
 template <class T>
-__global__ void __launch_bounds__(256) glu_align_kernel(const T* __restrict__ from, size_t ld_from, T* __restrict__ to, size_t ld_to, size_t rows, size_t cols) {
-    grid_release();
-    grid_wait();
-    const size_t vecs = ld_to / 8;
-    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < rows * vecs; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / vecs, c = (i % vecs) * 8;
-        Vec<T, 8> x;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.v[j] = c + j < cols ? from[r * ld_from + c + j] : from_f32<T>(0.0f);
-        *reinterpret_cast<Vec<T, 8>*>(to + r * ld_to + c) = x;
+__global__ void __launch_bounds__(128) glu_align_kernel(const __grid_constant__ AlignArgs a) {
+    const Operand& x = a.from[blockIdx.z];
+    const size_t c = (blockIdx.x * 128 + threadIdx.x) * 8, ld = a.ld_to[blockIdx.z];
+    if (c >= ld) return;
+    for (size_t r = blockIdx.y; r < x.rows; r += gridDim.y) {
+        const Vec<T, 8> v = load_any<T>(static_cast<const T*>(x.p) + r * x.ld + c, (unsigned)min((size_t)8, x.cols - c));
+        *reinterpret_cast<Vec<T, 8>*>(static_cast<T*>(a.to[blockIdx.z]) + r * ld + c) = v;
     }
 }
 
-struct Operand { const void* p; size_t ld; };
 bool copyable(const void* p, size_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+// Makes operands readable by tensor copies, those that are not through the workspace.
 template <class T>
-int align(Operand* x, size_t rows, size_t cols, Scratch* scratch, cudaStream_t s) {
-    const size_t ld = (cols + 7) / 8 * 8;
-    if (rows == 1) x->ld = ld;   // never used
-    if (copyable(x->p, x->ld)) return ZKB_OK;
-    T* to = scratch->get_n<T>(rows * ld);
-    if (!to) return ZKB_ERR_CUDA;
+int align(std::initializer_list<Operand*> operands, Scratch* scratch, cudaStream_t s) {
+    AlignArgs a = {};
+    unsigned n = 0, rows = 0, blocks = 0;
+    for (Operand* x : operands) {
+        const size_t ld = (x->cols + 7) / 8 * 8;
+        if (x->rows == 1) x->ld = ld;   // never used
+        if (copyable(x->p, x->ld)) continue;
+        a.from[n] = *x;
+        a.ld_to[n] = ld;
+        if (!(a.to[n] = scratch->get_n<T>(x->rows * ld))) return ZKB_ERR_CUDA;
+        x->p = a.to[n], x->ld = ld;
+        rows = std::max(rows, (unsigned)x->rows), blocks = std::max(blocks, div_up(ld, 8 * 128));
+        ++n;
+    }
+    if (!n) return ZKB_OK;
     const auto glu_align = glu_align_kernel<T>;
-    ZKB_TRY(launch_beside("glu_align", glu_align, (unsigned)std::min<size_t>((rows * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(x->p), x->ld, to, ld, rows,
-               cols));
-    *x = {to, ld};
+    ZKB_LAUNCH(glu_align, dim3(blocks, std::min(rows, std::max(1u, 32u * sm_count() / blocks)), n), 128, 0, s, a);
     return ZKB_OK;
 }
 
@@ -560,7 +623,10 @@ template <class T, class Args>
 int product_launch(const Args& p, size_t tiles, cudaStream_t s) {
     const auto glu_product = glu_product_kernel<T, Args>;
     ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kProductSmem));
-    return launch_beside("glu_product", glu_product, 2 * (unsigned)std::min(tiles, (size_t)sm_count() / 2), kProductThreads, kProductSmem, s, p);
+    // A plain launch, and no trigger in the kernel: small blocks of a successor that is launched beside it and waits for its end could take
+    // the SMs of a cluster that has no place yet, and neither would ever go on.
+    ZKB_LAUNCH(glu_product, 2 * (unsigned)std::min(tiles, (size_t)sm_count() / 2), kProductThreads, kProductSmem, s, p);
+    return ZKB_OK;
 }
 void lay_results(Results* r, size_t m, size_t n, unsigned tile_cols, size_t k) {
     r->m = (unsigned)m, r->n = (unsigned)n, r->slices = div_up(k, kDepth);
@@ -583,7 +649,7 @@ int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* fla
     const auto glu_few = glu_few_kernel<T, kTokens>;
     constexpr size_t smem = few_smem<kTokens>();
     ZKB_CUDA(cudaFuncSetAttribute(glu_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    ZKB_TRY(launch_beside("glu_few", glu_few, blocks, kProductThreads, smem, s, p));
+    ZKB_TRY(launch_beside("glu_few", glu_few, blocks, kFewThreads, smem, s, p));
     const FewEnd e = {p.parts, p.tokens, (unsigned)a.hidden, p.tiles, p.slices, blocks, {a.h, a.gate_out, a.up_out}, {a.ldh, a.ldg, a.ldu}, a.act};
     const auto glu_few_finish = glu_few_finish_kernel<T>;
     return launch_beside("glu_few_finish", glu_few_finish, dim3(p.tiles, p.tokens), kFewCols, 0, s, e);
@@ -592,15 +658,13 @@ int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* fla
 template <class T>
 int glu_launch(const GluArgs& a, cudaStream_t s) {
     if (!a.in) {   // a sum over nothing
-        for (auto [p, ld] : {Operand{a.h, a.ldh}, Operand{a.gate_out, a.ldg}, Operand{a.up_out, a.ldu}})
-            if (p) ZKB_CUDA(cudaMemset2DAsync(const_cast<void*>(p), ld * 2, 0, a.hidden * 2, a.tokens, s));
+        for (auto [p, ld] : {std::pair<void*, size_t>{a.h, a.ldh}, {a.gate_out, a.ldg}, {a.up_out, a.ldu}})
+            if (p) ZKB_CUDA(cudaMemset2DAsync(p, ld * 2, 0, a.hidden * 2, a.tokens, s));
         return ZKB_OK;
     }
     Scratch scratch(s);
-    Operand x = {a.x, a.ldx}, wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
-    ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
-    ZKB_TRY(align<T>(&wg, a.in, a.hidden, &scratch, s));
-    ZKB_TRY(align<T>(&wu, a.in, a.hidden, &scratch, s));
+    Operand x = {a.x, a.ldx, a.tokens, a.in}, wg = {a.wg, a.ldwg, a.in, a.hidden}, wu = {a.wu, a.ldwu, a.in, a.hidden};
+    ZKB_TRY(align<T>({&x, &wg, &wu}, &scratch, s));
     int* const flag = tc::wait_flag();
     if (!flag) return ZKB_ERR_CUDA;
     if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, flag, &scratch, s);
@@ -633,15 +697,18 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     T* dg = scratch.get_n<T>(a.tokens * ld);
     T* du = scratch.get_n<T>(a.tokens * ld);
     if (!dg || !du) return ZKB_ERR_CUDA;
-    const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, 8> : glu_split_kernel<T, 1>;
-    ZKB_TRY(launch_beside("glu_split", glu_split, (unsigned)std::min<size_t>((a.tokens * ld / 8 + 255) / 256, 16 * sm_count()), 256, 0, s, static_cast<const T*>(a.gate), a.ldg,
-               static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld, a.tokens, F, a.act));
+    const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, true> : glu_split_kernel<T, false>;
+    const unsigned across = div_up(F, 8 * 128);
+    ZKB_LAUNCH(glu_split, dim3(across, (unsigned)std::min<size_t>(a.tokens, std::max(1u, 32u * sm_count() / across))), 128, 0, s,
+                          static_cast<const T*>(a.gate), a.ldg, static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld,
+                          (unsigned)a.tokens, (unsigned)F, a.act);
+    Operand x = {a.x, a.ldx, a.tokens, a.in}, wg = {a.wg, a.ldwg, a.in, F}, wu = {a.wu, a.ldwu, a.in, F};
+    if (a.dx && a.dwg) ZKB_TRY(align<T>({&x, &wg, &wu}, &scratch, s));
+    else if (a.dx) ZKB_TRY(align<T>({&wg, &wu}, &scratch, s));
+    else ZKB_TRY(align<T>({&x}, &scratch, s));
     GradArgs p = {};
     if (!(p.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
     if (a.dx) {
-        Operand wg = {a.wg, a.ldwg}, wu = {a.wu, a.ldwu};
-        ZKB_TRY(align<T>(&wg, a.in, F, &scratch, s));
-        ZKB_TRY(align<T>(&wu, a.in, F, &scratch, s));
         ZKB_TRY(tc::make_map(&p.dg_rows[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
         ZKB_TRY(tc::make_map(&p.dg_rows[1], kCode<T>, du, a.tokens, F, ld, kHalf));
         ZKB_TRY(tc::make_map(&p.w[0], kCode<T>, wg.p, a.in, F, wg.ld, kHalf));
@@ -650,8 +717,6 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         set_result(&p.dx, 0, a.dx, a.lddx);
     }
     if (a.dwg) {
-        Operand x = {a.x, a.ldx};
-        ZKB_TRY(align<T>(&x, a.tokens, a.in, &scratch, s));
         ZKB_TRY(tc::make_map(&p.x, kCode<T>, x.p, a.tokens, a.in, x.ld, kDepth));
         ZKB_TRY(tc::make_map(&p.dg_cols[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
         ZKB_TRY(tc::make_map(&p.dg_cols[1], kCode<T>, du, a.tokens, F, ld, kDepth));
@@ -659,10 +724,22 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         set_result(&p.dw, 0, a.dwg, a.lddwg);
         set_result(&p.dw, 1, a.dwu, a.lddwu);
     }
-    const size_t longs = (size_t)p.dx.row_tiles * p.dx.col_tiles, shorts = 2 * (size_t)p.dw.row_tiles * p.dw.col_tiles;
+    // at least 8 slices to a part: fewer cost more in the sums' way through memory than they save
+    const size_t whole = (size_t)p.dx.row_tiles * p.dx.col_tiles, most = sm_count() / 2;
+    p.parts = whole && whole < most ? (unsigned)std::max<size_t>(1, std::min<size_t>(most / whole, 2 * p.dx.slices / 8)) : 1;
+    if (p.parts > 1) {
+        p.sums_ld = (p.dx.n + 3) / 4 * 4;
+        p.sums = scratch.get_n<float>((size_t)p.parts * p.dx.m * p.sums_ld);
+        if (!p.sums) return ZKB_ERR_CUDA;
+    }
+    const size_t longs = whole * p.parts, shorts = 2 * (size_t)p.dw.row_tiles * p.dw.col_tiles;
     const size_t pairs = std::min(longs + shorts, (size_t)sm_count() / 2), spare = pairs - longs % pairs;
-    if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((2 * p.dx.slices + p.dw.slices / 2) / p.dw.slices, shorts / spare);
-    return product_launch<T>(p, longs + shorts, s);
+    if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((2 * p.dx.slices / p.parts + p.dw.slices / 2) / p.dw.slices, shorts / spare);
+    ZKB_TRY(product_launch<T>(p, longs + shorts, s));
+    if (p.parts == 1) return ZKB_OK;
+    const auto glu_add_parts = p.dx.wide[0] ? glu_add_parts_kernel<T, true> : glu_add_parts_kernel<T, false>;
+    ZKB_LAUNCH(glu_add_parts, dim3(div_up(p.dx.n, 4 * 128), p.dx.m), 128, 0, s, p.sums, p.parts, p.dx.m, p.dx.n, p.sums_ld, static_cast<T*>(a.dx), a.lddx);
+    return ZKB_OK;
 }
 
 int check_matrix(const char* who, const char* name, const void* p, size_t rows, size_t cols, size_t ld, bool needed) {

@@ -57,6 +57,21 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, cons
     *reinterpret_cast<volatile int*>(w.flag) = 1;
     return false;
 }
+// The same by a whole warp, which stays together: instructions on tensor memory follow that all its lanes have to reach as one.
+__device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity, const Watch& w) {
+    unsigned long long start = 0;
+    for (unsigned i = 0; i < (1u << 28); ++i) {
+        if (__all_sync(0xffffffffu, barrier_done(bar, parity))) return true;
+        if ((i & 63) != 63) continue;
+        const unsigned long long t = now_ns();
+        if (!start) start = t;
+        if (__any_sync(0xffffffffu, *w.dead || t - start > 2000000000ull)) break;
+    }
+    *w.dead = 1;
+    *reinterpret_cast<volatile int*>(w.flag) = 1;
+    __syncwarp();
+    return false;
+}
 // some milliseconds: long after the copies and products that a block has in flight
 __device__ __forceinline__ void pause() {
     const unsigned long long start = now_ns();
@@ -116,16 +131,20 @@ __device__ __forceinline__ void load_bytes(uint32_t dst, unsigned long long src,
 
 // ---- tcgen05 -----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t at, uint32_t cols) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+    __syncwarp();
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t at, uint32_t cols) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tmem_free_pair(uint32_t tmem, uint32_t cols) {
+    __syncwarp();
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
 }
