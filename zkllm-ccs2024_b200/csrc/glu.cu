@@ -91,8 +91,7 @@ struct Results {
     unsigned m, n;                           // of one result (gated: hidden)
     unsigned row_tiles, col_tiles, slices;   // its tiles, and slices of 64 of one sum
     void* out[3];                            // gated: h, gate, up (or null); summed: dx; paired: dw_gate, dw_up
-    size_t ld[3];
-    bool wide[3];                            // 16-byte stores
+    size_t ld[3];                            // addresses and row strides are whole 16 bytes
 };
 struct GatedArgs {
     CUtensorMap a, b[2];
@@ -113,8 +112,7 @@ struct Tile { unsigned row, col, pair, part, from, to; bool paired; };   // from
 
 // 32 x 32 values of a warp (row i with lane i) to rows row0.. and columns col0.. of a matrix of m x n.
 template <class T>
-__device__ __forceinline__ void store_block(char* stage, const float (&v)[32], T* out, size_t ld, bool wide, unsigned row0, unsigned col0, unsigned m,
-                                            unsigned n) {
+__device__ __forceinline__ void store_block(char* stage, const float (&v)[32], T* out, size_t ld, unsigned row0, unsigned col0, unsigned m, unsigned n) {
     const unsigned lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
@@ -124,25 +122,17 @@ __device__ __forceinline__ void store_block(char* stage, const float (&v)[32], T
         *reinterpret_cast<Vec<T, 8>*>(stage + lane * 80 + i * 2) = x;
     }
     __syncwarp();
-    if (wide) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned r = i * 8 + lane / 4, c = (lane % 4) * 8;
-            const Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8>*>(stage + r * 80 + c * 2);
-            if (row0 + r >= m) continue;
-            T* to = out + (size_t)(row0 + r) * ld + col0 + c;
-            if (col0 + c + 8 <= n) {
-                *reinterpret_cast<Vec<T, 8>*>(to) = x;
-            } else {
-                for (unsigned j = 0; col0 + c + j < n && j < 8; ++j) to[j] = x.v[j];
-            }
+    for (int i = 0; i < 4; ++i) {
+        const unsigned r = i * 8 + lane / 4, c = (lane % 4) * 8;
+        const Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8>*>(stage + r * 80 + c * 2);
+        if (row0 + r >= m) continue;
+        T* to = out + (size_t)(row0 + r) * ld + col0 + c;
+        if (col0 + c + 8 <= n) {
+            *reinterpret_cast<Vec<T, 8>*>(to) = x;
+        } else {
+            for (unsigned j = 0; col0 + c + j < n && j < 8; ++j) to[j] = x.v[j];
         }
-    } else {
-        T* to = out + (size_t)row0 * ld + col0 + lane;
-        const unsigned rows = col0 + lane < n && row0 < m ? min(32u, m - row0) : 0;
-#pragma unroll 8
-        for (unsigned r = 0; r < 32; ++r)
-            if (r < rows) to[r * ld] = *reinterpret_cast<const T*>(stage + r * 80 + lane * 2);
     }
     __syncwarp();
 }
@@ -294,11 +284,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
                     tc::load_columns(from + kHalf + c, u);
                     const unsigned col0 = t.col * kHalf + c;
                     if (r.out[1]) {
-                        store_block<T>(stage, g, static_cast<T*>(r.out[1]), r.ld[1], r.wide[1], row0, col0, r.m, r.n);
-                        store_block<T>(stage, u, static_cast<T*>(r.out[2]), r.ld[2], r.wide[2], row0, col0, r.m, r.n);
+                        store_block<T>(stage, g, static_cast<T*>(r.out[1]), r.ld[1], row0, col0, r.m, r.n);
+                        store_block<T>(stage, u, static_cast<T*>(r.out[2]), r.ld[2], row0, col0, r.m, r.n);
                     }
                     gate(p.act, g, u);
-                    store_block<T>(stage, g, static_cast<T*>(r.out[0]), r.ld[0], r.wide[0], row0, col0, r.m, r.n);
+                    store_block<T>(stage, g, static_cast<T*>(r.out[0]), r.ld[0], row0, col0, r.m, r.n);
                 }
             } else {
                 for (unsigned c = 0; c < kTile; c += 32) {
@@ -314,7 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
                         __syncwarp();   // the next columns are read by the warp as one
                         continue;
                     }
-                    store_block<T>(stage, v, static_cast<T*>(r.out[t.pair]), r.ld[t.pair], r.wide[t.pair], row0, col0, r.m, r.n);
+                    store_block<T>(stage, v, static_cast<T*>(r.out[t.pair]), r.ld[t.pair], row0, col0, r.m, r.n);
                 }
             }
             tc::fence_before_sync();
@@ -596,6 +586,30 @@ __global__ void __launch_bounds__(128) glu_align_kernel(const __grid_constant__ 
     }
 }
 
+// Results for addresses that take no 16-byte stores are formed in the workspace and brought to their places by 16-byte granules of
+// the place; a row's first and last are written by value.
+struct PlaceArgs {
+    const void* from[3];
+    void* to[3];
+    size_t ld_from[3], ld_to[3];
+    unsigned rows, cols;
+};
+template <class T>
+__global__ void __launch_bounds__(128) glu_place_kernel(const __grid_constant__ PlaceArgs a) {
+    const int g = blockIdx.x * 128 + threadIdx.x, cols = (int)a.cols;
+    for (size_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        const T* from = static_cast<const T*>(a.from[blockIdx.z]) + r * a.ld_from[blockIdx.z];
+        T* to = static_cast<T*>(a.to[blockIdx.z]) + r * a.ld_to[blockIdx.z];
+        const int e = g * 8 - (int)((reinterpret_cast<uintptr_t>(to) & 15) / 2);   // the granule's first value
+        if (e >= cols) continue;
+        if (e >= 0 && e + 8 <= cols) {
+            *reinterpret_cast<Vec<T, 8>*>(to + e) = load_any<T>(from + e, 8);
+        } else {
+            for (int j = max(e, 0); j < min(e + 8, cols); ++j) to[j] = from[j];
+        }
+    }
+}
+
 bool copyable(const void* p, size_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
 // Makes operands readable by tensor copies, those that are not through the workspace.
 template <class T>
@@ -632,7 +646,27 @@ void lay_results(Results* r, size_t m, size_t n, unsigned tile_cols, size_t k) {
     r->m = (unsigned)m, r->n = (unsigned)n, r->slices = div_up(k, kDepth);
     r->row_tiles = div_up(m, kTile), r->col_tiles = div_up(n, tile_cols);
 }
-void set_result(Results* r, int i, void* out, size_t ld) { r->out[i] = out, r->ld[i] = ld, r->wide[i] = copyable(out, ld); }
+// Sets a result's place, or room for it in the workspace and a note of where it goes.
+template <class T>
+int set_result(Results* r, int i, void* out, size_t ld, Scratch* scratch, PlaceArgs* later, unsigned* n) {
+    r->out[i] = out, r->ld[i] = ld;
+    if (!out || copyable(out, ld)) return ZKB_OK;
+    r->ld[i] = (r->n + 7) / 8 * 8;
+    if (!(r->out[i] = scratch->get_n<T>((size_t)r->m * r->ld[i]))) return ZKB_ERR_CUDA;
+    later->from[*n] = r->out[i], later->ld_from[*n] = r->ld[i];
+    later->to[*n] = out, later->ld_to[*n] = ld;
+    later->rows = r->m, later->cols = r->n;
+    ++*n;
+    return ZKB_OK;
+}
+template <class T>
+int place_results(const PlaceArgs& a, unsigned n, cudaStream_t s) {
+    if (!n) return ZKB_OK;
+    const unsigned across = div_up(a.cols + 7, 8 * 128);
+    const auto glu_place = glu_place_kernel<T>;
+    ZKB_LAUNCH(glu_place, dim3(across, std::min(a.rows, std::max(1u, 32u * sm_count() / across)), n), 128, 0, s, a);
+    return ZKB_OK;
+}
 
 template <class T> constexpr int kCode = std::is_same<T, __half>::value ? ZKB_F16 : ZKB_BF16;
 
@@ -677,10 +711,13 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     ZKB_TRY(tc::make_map(&p.b[0], kCode<T>, wg.p, a.in, a.hidden, wg.ld, kDepth));
     ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
     lay_results(&p.r, a.tokens, a.hidden, kHalf, a.in);
-    set_result(&p.r, 0, a.h, a.ldh);
-    set_result(&p.r, 1, a.gate_out, a.ldg);
-    set_result(&p.r, 2, a.up_out, a.ldu);
-    return product_launch<T>(p, (size_t)p.r.row_tiles * p.r.col_tiles, s);
+    PlaceArgs later = {};
+    unsigned n = 0;
+    ZKB_TRY(set_result<T>(&p.r, 0, a.h, a.ldh, &scratch, &later, &n));
+    ZKB_TRY(set_result<T>(&p.r, 1, a.gate_out, a.ldg, &scratch, &later, &n));
+    ZKB_TRY(set_result<T>(&p.r, 2, a.up_out, a.ldu, &scratch, &later, &n));
+    ZKB_TRY(product_launch<T>(p, (size_t)p.r.row_tiles * p.r.col_tiles, s));
+    return place_results<T>(later, n, s);
 }
 
 template <class T>
@@ -707,6 +744,8 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     else if (a.dx) ZKB_TRY(align<T>({&wg, &wu}, &scratch, s));
     else ZKB_TRY(align<T>({&x}, &scratch, s));
     GradArgs p = {};
+    PlaceArgs later_dx = {}, later_dw = {};
+    unsigned n_dx = 0, n_dw = 0;
     if (!(p.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
     if (a.dx) {
         ZKB_TRY(tc::make_map(&p.dg_rows[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
@@ -714,15 +753,14 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         ZKB_TRY(tc::make_map(&p.w[0], kCode<T>, wg.p, a.in, F, wg.ld, kHalf));
         ZKB_TRY(tc::make_map(&p.w[1], kCode<T>, wu.p, a.in, F, wu.ld, kHalf));
         lay_results(&p.dx, a.tokens, a.in, kTile, F);
-        set_result(&p.dx, 0, a.dx, a.lddx);
     }
     if (a.dwg) {
         ZKB_TRY(tc::make_map(&p.x, kCode<T>, x.p, a.tokens, a.in, x.ld, kDepth));
         ZKB_TRY(tc::make_map(&p.dg_cols[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
         ZKB_TRY(tc::make_map(&p.dg_cols[1], kCode<T>, du, a.tokens, F, ld, kDepth));
         lay_results(&p.dw, a.in, F, kTile, a.tokens);
-        set_result(&p.dw, 0, a.dwg, a.lddwg);
-        set_result(&p.dw, 1, a.dwu, a.lddwu);
+        ZKB_TRY(set_result<T>(&p.dw, 0, a.dwg, a.lddwg, &scratch, &later_dw, &n_dw));
+        ZKB_TRY(set_result<T>(&p.dw, 1, a.dwu, a.lddwu, &scratch, &later_dw, &n_dw));
     }
     // at least 8 slices to a part: fewer cost more in the sums' way through memory than they save
     const size_t whole = (size_t)p.dx.row_tiles * p.dx.col_tiles, most = sm_count() / 2;
@@ -731,13 +769,19 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         p.sums_ld = (p.dx.n + 3) / 4 * 4;
         p.sums = scratch.get_n<float>((size_t)p.parts * p.dx.m * p.sums_ld);
         if (!p.sums) return ZKB_ERR_CUDA;
+    } else if (a.dx) {
+        ZKB_TRY(set_result<T>(&p.dx, 0, a.dx, a.lddx, &scratch, &later_dx, &n_dx));
     }
     const size_t longs = whole * p.parts, shorts = 2 * (size_t)p.dw.row_tiles * p.dw.col_tiles;
-    const size_t pairs = std::min(longs + shorts, (size_t)sm_count() / 2), spare = pairs - longs % pairs;
-    if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((2 * p.dx.slices / p.parts + p.dw.slices / 2) / p.dw.slices, shorts / spare);
+    const size_t pairs = std::min(longs + shorts, most), spare = pairs - longs % pairs;
+    // A tile costs its slices, but no less than the 16 slices' time that taking it out takes.
+    const unsigned cost_long = std::max(16u, 2 * p.dx.slices / p.parts), cost_short = std::max(16u, p.dw.slices);
+    if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((cost_long + cost_short / 2) / cost_short, shorts / spare);
     ZKB_TRY(product_launch<T>(p, longs + shorts, s));
+    ZKB_TRY(place_results<T>(later_dx, n_dx, s));
+    ZKB_TRY(place_results<T>(later_dw, n_dw, s));
     if (p.parts == 1) return ZKB_OK;
-    const auto glu_add_parts = p.dx.wide[0] ? glu_add_parts_kernel<T, true> : glu_add_parts_kernel<T, false>;
+    const auto glu_add_parts = copyable(a.dx, a.lddx) ? glu_add_parts_kernel<T, true> : glu_add_parts_kernel<T, false>;
     ZKB_LAUNCH(glu_add_parts, dim3(div_up(p.dx.n, 4 * 128), p.dx.m), 128, 0, s, p.sums, p.parts, p.dx.m, p.dx.n, p.sums_ld, static_cast<T*>(a.dx), a.lddx);
     return ZKB_OK;
 }
