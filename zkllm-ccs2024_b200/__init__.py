@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -66,10 +67,14 @@ class RopeTensor(ctypes.Structure):
         (f"{side}_{axis}", ctypes.c_int64) for side in ("in", "out") for axis in ("batch", "token", "head")]
 
 
+_ROPE_PACK = struct.Struct("=QQQ6q").pack
+
+
 def rope_tensors(*tensors):
     """The array of tensors that zkb_rope takes, each given as (address in, address out, heads, strides in, strides out)
     with the strides of batch, token and head in elements."""
-    return (RopeTensor * len(tensors))(*(RopeTensor(i, o, h, *si, *so) for i, o, h, si, so in tensors))
+    packed = b"".join(_ROPE_PACK(i or 0, o or 0, h, *si, *so) for i, o, h, si, so in tensors)
+    return (RopeTensor * len(tensors)).from_buffer_copy(packed)
 
 
 def exported_symbols_from_header() -> list:

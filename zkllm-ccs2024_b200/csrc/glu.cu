@@ -69,7 +69,7 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 // Bound by the tensor cores.  Persistent pairs of blocks (one block per SM) work through 256 x 256 tiles.  Each block holds 128 rows of the
 // first operand and 128 columns of the second, so that a slice costs both SMs together 64 KB of copies and shared memory where two
 // blocks on their own would need 96.  In each block warp 0 copies 64-deep slices into a ring; in the first, warp 1 issues
-// the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 7 of both take their 128 rows of the other
+// the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 11 of both take their 128 rows of the other
 // accumulator out, so that a tile's epilogue runs beside the next tile's products.
 //
 // The forms of a tile:
@@ -81,7 +81,7 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 // the rest are dealt out to all, so that all end together.  Where dx has fewer tiles than there are pairs, each of its sums is cut
 // into parts, which are left in 32 bits and added in order by glu_add_parts_kernel.
 constexpr int kTile = 256, kHalf = 128, kDepth = 64;
-constexpr int kTakers = 4;             // epilogue warps of a block (8 were no faster)
+constexpr int kTakers = 8;             // epilogue warps of a block, two to 32 rows: with 4 a tile of few slices waits for its way out
 constexpr int kProductThreads = 128 + 32 * kTakers;
 constexpr int kStageBytes = 32 * 80;   // an epilogue warp's 32 x 32 values on their way out, rows 80 bytes apart
 constexpr int kRing = 6, kSlice = 2 * kHalf * kDepth * 2;
@@ -269,6 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
         }
     } else if (warp >= 4) {
         char* stage = stages + (warp - 4) * kStageBytes;
+        const unsigned side = (warp - 4) / 4;
         Tile t;
         for (unsigned i = 0; tile_of(p, i, first, step, &t); ++i) {
             const unsigned acc = i & 1;
@@ -278,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
             const unsigned row0 = t.row * kTile + rank * kHalf + warp % 4 * 32;
             const Results& r = results_of(p, t);
             if constexpr (kGated) {
-                for (unsigned c = 0; c < kHalf; c += 32) {
+                for (unsigned c = side * (kHalf / 2); c < (side + 1) * (kHalf / 2); c += 32) {
                     float g[32], u[32];
                     tc::load_columns(from + c, g);
                     tc::load_columns(from + kHalf + c, u);
@@ -291,7 +292,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
                     store_block<T>(stage, g, static_cast<T*>(r.out[0]), r.ld[0], row0, col0, r.m, r.n);
                 }
             } else {
-                for (unsigned c = 0; c < kTile; c += 32) {
+                for (unsigned c = side * (kTile / 2); c < (side + 1) * (kTile / 2); c += 32) {
                     float v[32];
                     tc::load_columns(from + c, v);
                     const unsigned col0 = t.col * kTile + c;
