@@ -707,3 +707,149 @@ def test_another_devices_memory_is_refused(zkb):
     with pytest.raises(zkb.ZkbError) as e:
         norm_call(zkb, 0, 0, x, None, False, None, "none", None, 1.0, None, 1e-5, None, torch.zeros(2, 8, device="cuda:0"), None, None, st=0)
     assert e.value.code == zkb.ERR_ARG
+
+
+def test_pinned_host_memory_is_refused(zkb):
+    x = torch.zeros(2, 8).pin_memory()
+    out = torch.zeros(2, 8, device="cuda")
+    with pytest.raises(zkb.ZkbError) as e:
+        norm_call(zkb, 0, 0, x, None, False, None, "none", None, 1.0, None, 1e-5, None, out, None, None)
+    assert e.value.code == zkb.ERR_ARG
+
+
+@pytest.mark.parametrize("n,e,f", [(4400, 72, 1100), (2560, 2048, 264), (2700, 1800, 520)])
+def test_glu_many_tiles(zkb, n, e, f):
+    """more rows of tiles than a band holds; more long tiles of dx than pairs of blocks, beside short ones of the weights"""
+    t = torch.bfloat16
+    x, wg, wu, gate, up, dh = glu_inputs(n, e, f, t, n)
+    h, g, u = (torch.empty(n, f, device="cuda", dtype=t) for _ in range(3))
+    glu_call(zkb, 2, "gelu", x, wg, wu, h, g, u)
+    check_glu(zkb, "bf16", "gelu", x, wg, wu, h, g, u)
+    dx, dwg, dwu = torch.full_like(x, math.nan), torch.full_like(wg, math.nan), torch.full_like(wu, math.nan)
+    glu_back_call(zkb, 2, "gelu", x, wg, wu, gate, up, dh, dx, dwg, dwu)
+    check_glu_back(zkb, "bf16", "gelu", x, wg, wu, gate, up, dh, dx, dwg, dwu)
+
+
+@pytest.mark.parametrize("rows,cols", [(5000, 96), (700, 4100), (310, 6000), (200, 12000), (160, 16384)])
+def test_block_norm_many_rows(zkb, rows, cols):
+    """more rows than resident blocks times slots, in each of the kernels' layouts, aligned and not: the ring goes round"""
+    for t, code, shift in ((torch.bfloat16, 2, 0), (torch.float32, 0, 0), (torch.float16, 1, 1)):
+        if cols + shift > 16384:     # refused: beyond the documented limit
+            continue
+        r, y, pg, wg, gv, dz, dr = norm_inputs(rows, cols + shift, t, t, "element", True, rows + cols)
+        x = r
+        ro, zz, inv = torch.empty(rows, cols + shift, device="cuda", dtype=t), torch.empty(rows, cols + shift, device="cuda", dtype=t), torch.empty(rows, device="cuda")
+        norm_call(zkb, code, code, x, y, True, pg, "element", gv, 0.7, wg, 1e-5, ro, zz, None, inv)
+        X, Y, PG, WG, GV = wide(x, y, pg, wg, gv)
+        br = branch_of(Y, PG, True, GV, "element", 0.7, 1e-5)
+        R = X + br
+        rinv = 1 / (R.pow(2).mean(1, keepdim=True) + 1e-5).sqrt()
+        k = norm_slack(cols + shift)
+        near(ro, R, t, k * (X.abs() + br.abs()))
+        near(zz, R * rinv * WG, t, 3 * k * (X.abs() + br.abs()) * rinv * WG.abs() + 3 * k * (R * rinv * WG).abs())
+        near(inv, rinv[:, 0], torch.float32, 3 * k * rinv[:, 0])
+        outs = [torch.full_like(r, math.nan), torch.full_like(y, math.nan), torch.full_like(gv, math.nan), torch.full_like(pg, math.nan), torch.full_like(wg, math.nan)]
+        back_call(zkb, code, code, r, y, True, pg, "element", gv, 0.7, wg, 1e-5, dz, dr, *outs)
+        want, _ = norm_grads(X - br, y, pg, wg, gv, "element", True, 0.7, 1e-5, dz, dr)   # the stream before the branch, so that r is the sum
+        R = X
+        rinv = 1 / (R.pow(2).mean(1, keepdim=True) + 1e-5).sqrt()
+        p = (dz.double() * WG).abs()
+        d = dr.double().abs() + rinv * (p + R.abs() * rinv.pow(2) * (p * R.abs()).mean(1, keepdim=True))
+        yinv = 1 / (Y.pow(2).mean(1, keepdim=True) + 1e-5).sqrt()
+        q = 0.7 * GV.abs() * d * PG.abs()
+        near(outs[0], want["x"], t, 8 * k * d)
+        near(outs[1], want["y"], t, 8 * k * yinv * (q + Y.abs() * yinv.pow(2) * (q * Y.abs()).mean(1, keepdim=True)))
+        near(outs[2], want["gv"], t, 8 * k * 0.7 * d * Y.abs() * yinv * PG.abs())
+        near(outs[3], want["pg"], t, 8 * norm_slack(rows + cols) * (0.7 * GV.abs() * d * Y.abs() * yinv).sum(0))
+        near(outs[4], want["wg"], t, 8 * norm_slack(rows + cols) * (dz.double() * R * rinv).abs().sum(0))
+        again = [torch.empty_like(o) for o in outs]
+        back_call(zkb, code, code, r, y, True, pg, "element", gv, 0.7, wg, 1e-5, dz, dr, *again)
+        assert all(torch.equal(a, b) for a, b in zip(again, outs))
+
+
+def test_two_host_threads_at_once(zkb):
+    """calls of two threads on streams and data of their own, interleaved as they come"""
+    import threading
+    t = torch.bfloat16
+    sets, errors = [], []
+    for seed in (1, 2):
+        x, wg, wu, gate, up, dh = glu_inputs(150, 264, 520, t, seed)
+        r, y, pg, gg, gv, dz, dr = norm_inputs(600, 1032, t, t, "channel", True, seed)
+        outs = [torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)]
+        nouts = [torch.empty_like(r), torch.empty_like(r), torch.empty_like(gv), torch.empty_like(pg), torch.empty_like(gg)]
+        h = torch.empty(9, 520, device="cuda", dtype=t)
+        sets.append((x, wg, wu, gate, up, dh, r, y, pg, gg, gv, dz, dr, outs, nouts, h))
+
+    def once(s, st):
+        x, wg, wu, gate, up, dh, r, y, pg, gg, gv, dz, dr, outs, nouts, h = s
+        glu_back_call(zkb, 2, "silu", x, wg, wu, gate, up, dh, *outs, st=st)
+        back_call(zkb, 2, 2, r, y, True, pg, "channel", gv, 0.7, gg, 1e-5, dz, dr, *nouts, st=st)
+        glu_call(zkb, 2, "silu", x[:9], wg, wu, h, None, None, st=st)
+    for s in sets:
+        once(s, stream())
+    torch.cuda.synchronize()
+    want = [[o.clone() for o in s[13] + s[14] + [s[15]]] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+
+    def work(s, st):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(30):
+                once(s, st.cuda_stream)
+            st.synchronize()
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in zip(sets, streams)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(s[13] + s[14] + [s[15]], w))
+
+
+def test_a_capture_may_hold_the_first_call(tmp_path):
+    """in a process of its own, the first call of each operator is made while its stream is captured"""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from tests import test_gpu_floatops as T
+from tests.conftest import load_package
+z = load_package()
+t = torch.bfloat16
+x, wg, wu, gate, up, dh = T.glu_inputs(200, 136, 328, t, 1)
+r, y, pg, gg, gv, dz, dr = T.norm_inputs(300, 520, t, t, "channel", True, 1)
+h, h9 = torch.zeros(200, 328, device="cuda", dtype=t), torch.zeros(9, 328, device="cuda", dtype=t)
+outs = [torch.zeros_like(x), torch.zeros_like(wg), torch.zeros_like(wu)]
+nouts = [torch.zeros_like(r), torch.zeros_like(r), torch.zeros_like(gv), torch.zeros_like(pg), torch.zeros_like(gg)]
+zz, rr = torch.zeros_like(r), torch.zeros_like(r)
+q = torch.randn(1, 200, 2, 64, device="cuda", dtype=t)
+qo, freq = torch.zeros_like(q), T.rope_freq(64)
+def go():
+    T.glu_call(z, 2, "silu", x, wg, wu, h, None, None)
+    T.glu_call(z, 2, "silu", x[:9], wg, wu, h9, None, None)
+    T.glu_back_call(z, 2, "silu", x, wg, wu, gate, up, dh, *outs)
+    T.norm_call(z, 2, 2, r, y, True, pg, "channel", gv, 0.7, gg, 1e-5, rr, zz, None, None)
+    T.back_call(z, 2, 2, r, y, True, pg, "channel", gv, 0.7, gg, 1e-5, dz, dr, *nouts)
+    T.rope_call(z, 2, [(q, qo)], 1, 200, 64, 64, False, freq, 1.0, None, 0, 5, False)
+torch.cuda.synchronize()
+g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(g, stream=st):
+    go()
+everything = [h, h9, rr, zz, qo] + outs + nouts
+g.replay()
+torch.cuda.synchronize()
+first = [o.clone() for o in everything]
+go()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(first, everything)) and all(a.any() for a in first)
+print("same")
+""".format(root=str(root))
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=root)
+    assert res.returncode == 0 and "same" in res.stdout, res.stdout[-1000:] + res.stderr[-3000:]

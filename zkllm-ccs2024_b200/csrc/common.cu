@@ -80,7 +80,7 @@ int check_device(const void* p, size_t align, const char* what) {
         cudaGetLastError();
         return fail(ZKB_ERR_ARG, std::string(what) + ": not an address that the device knows");
     }
-    if (at.type == cudaMemoryTypeUnregistered) return fail(ZKB_ERR_ARG, std::string(what) + ": pageable host memory");
+    if (at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) return fail(ZKB_ERR_ARG, std::string(what) + ": host memory");
     if (at.type == cudaMemoryTypeDevice && at.device != dev) return fail(ZKB_ERR_ARG, std::string(what) + ": memory of another device");
     return ZKB_OK;
 }
@@ -132,6 +132,7 @@ static cudaMemPool_t library_pool() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lk(mu);
     if (!made[dev]) {
+        const SetupDuringCapture setup;
         cudaMemPoolProps props;
         memset(&props, 0, sizeof(props));
         props.allocType = cudaMemAllocationTypePinned;

@@ -71,6 +71,17 @@ inline cudaStream_t as_stream(void* s) {
     return s ? reinterpret_cast<cudaStream_t>(s) : g_default_stream.load(std::memory_order_relaxed);
 }
 
+// For the length of a block, calls that set something up once (a memory pool, page-locked memory) are allowed although
+// a stream of the process is being captured: they are no part of what is captured.
+class SetupDuringCapture {
+public:
+    SetupDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+    ~SetupDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+
+private:
+    cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+};
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

@@ -812,12 +812,9 @@ static std::mutex g_wait_mutex;
 int* wait_flag() {
     std::lock_guard<std::mutex> lock(g_wait_mutex);
     if (!g_wait_flag) {
-        // the first call may be inside another stream's capture, which forbids allocations by default
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);
+        const SetupDuringCapture setup;
         void* p = nullptr;
         const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-        cudaThreadExchangeStreamCaptureMode(&mode);
         if (e != cudaSuccess) {
             cuda_fail(e, "cudaHostAlloc(wait flag)");
             return nullptr;
