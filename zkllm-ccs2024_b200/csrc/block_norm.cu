@@ -715,15 +715,14 @@ int check_common(const char* who, int dtype, int gains_dtype, size_t rows, size_
 struct Matrix { const void* p; size_t ld; const char* name; };
 int check_matrix(const char* who, const Matrix& m, int dtype, size_t rows, size_t cols, bool* wide) {
     if (!m.p) return ZKB_OK;
-    const std::string w = std::string(who) + ": " + m.name;
-    if (m.ld < cols && rows > 1) return fail(ZKB_ERR_DIM, w + ": row stride below the row's length");
-    ZKB_TRY(check_device(m.p, type_size(dtype), w.c_str()));
+    if (m.ld < cols && rows > 1) return fail(ZKB_ERR_DIM, std::string(who) + ": " + m.name + ": row stride below the row's length");
+    ZKB_TRY(check_device(m.p, type_size(dtype), who, m.name));
     if (!aligned_to(m.p, 16) || (m.ld * type_size(dtype)) % 16) *wide = false;
     return ZKB_OK;
 }
 int check_vector(const char* who, const void* p, const char* name, int dtype, bool* wide) {
     if (!p) return ZKB_OK;
-    ZKB_TRY(check_device(p, type_size(dtype), (std::string(who) + ": " + name).c_str()));
+    ZKB_TRY(check_device(p, type_size(dtype), who, name));
     if (!aligned_to(p, 16)) *wide = false;
     return ZKB_OK;
 }

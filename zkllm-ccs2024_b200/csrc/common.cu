@@ -70,18 +70,19 @@ int sm_count() {
     return cached[dev];
 }
 
-int check_device(const void* p, size_t align, const char* what) {
+int check_device(const void* p, size_t align, const char* who, const char* what) {
     if (!p) return ZKB_OK;
-    if (!aligned_to(p, align)) return fail(ZKB_ERR_ARG, std::string(what) + ": address is not a multiple of the element size");
+    const auto refuse = [&](const char* why) { return fail(ZKB_ERR_ARG, std::string(who) + ": " + what + ": " + why); };
+    if (!aligned_to(p, align)) return refuse("address is not a multiple of the element size");
     cudaPointerAttributes at;
     int dev = 0;
     ZKB_CUDA(cudaGetDevice(&dev));
     if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
         cudaGetLastError();
-        return fail(ZKB_ERR_ARG, std::string(what) + ": not an address that the device knows");
+        return refuse("not an address that the device knows");
     }
-    if (at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) return fail(ZKB_ERR_ARG, std::string(what) + ": host memory");
-    if (at.type == cudaMemoryTypeDevice && at.device != dev) return fail(ZKB_ERR_ARG, std::string(what) + ": memory of another device");
+    if (at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) return refuse("host memory");
+    if (at.type == cudaMemoryTypeDevice && at.device != dev) return refuse("memory of another device");
     return ZKB_OK;
 }
 

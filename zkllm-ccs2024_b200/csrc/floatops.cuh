@@ -44,7 +44,7 @@ inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintpt
 
 // A pointer argument of the float operators: where it is given it has to be a whole element's address and memory that the
 // current device reaches, so that a host array or another device's tensor ends in an error and not in a fault.
-int check_device(const void* p, size_t align, const char* what);
+int check_device(const void* p, size_t align, const char* who, const char* what);
 
 // A kernel that was launched beside its predecessor waits for that one's end and results; a kernel lets its successor be launched.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -79,7 +79,7 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 // The gradients' launch holds tiles of both of the last: the few, long tiles of dx first, one or two to a pair of blocks, and the
 // many short ones of the weights where there is room.  The pairs with one tile of dx less take `head` of the short ones each before
 // the rest are dealt out to all, so that all end together.  Where dx has fewer tiles than there are pairs, each of its sums is cut
-// into parts, which are left in 32 bits and added in order by glu_add_parts_kernel.
+// into parts, which are left in 32 bits and added in order by glu_after_kernel.
 constexpr int kTile = 256, kHalf = 128, kDepth = 64;
 constexpr int kTakers = 8;             // epilogue warps of a block, two to 32 rows: with 4 a tile of few slices waits for its way out
 constexpr int kProductThreads = 128 + 32 * kTakers;
@@ -512,50 +512,65 @@ __device__ __forceinline__ Vec<T, 8> load_any(const T* p, unsigned count) {
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
 // follow have to be: each is off by half a step at most, independently, so a sum over them is off by no more, relative to its
 // norm, than its own rounding.
-template <class T, bool kWidePath>
-__global__ void __launch_bounds__(128) glu_split_kernel(const T* __restrict__ gate, size_t ldg, const T* __restrict__ up, size_t ldu, const T* __restrict__ dh,
-                                                        size_t ldh, T* __restrict__ dg, T* __restrict__ du, size_t ld, unsigned rows, unsigned cols, int act) {
+struct SplitArgs {
+    const void *gate, *up, *dh;
+    void *dg, *du;
+    size_t ldg, ldu, ldh, ld;
+    unsigned rows, cols;   // no rows: nothing to split
+    int act;
+    bool wide;
+};
+template <class T>
+__device__ __forceinline__ void split_rows(const SplitArgs& a) {
     const unsigned n = (blockIdx.x * 128 + threadIdx.x) * 8;
-    if (n >= cols) return;
-    for (unsigned m = blockIdx.y; m < rows; m += gridDim.y) {
+    if (n >= a.cols) return;
+    for (unsigned m = blockIdx.y; m < a.rows; m += gridDim.y) {
+        const T *gate = static_cast<const T*>(a.gate) + m * a.ldg + n, *up = static_cast<const T*>(a.up) + m * a.ldu + n,
+                *dh = static_cast<const T*>(a.dh) + m * a.ldh + n;
         float g[8], u[8], d[8];
-        if (kWidePath && n + 8 <= cols) {
-            load_vec<T, 8>(gate + m * ldg + n, g);
-            load_vec<T, 8>(up + m * ldu + n, u);
-            load_vec<T, 8>(dh + m * ldh + n, d);
+        if (a.wide && n + 8 <= a.cols) {
+            load_vec<T, 8>(gate, g);
+            load_vec<T, 8>(up, u);
+            load_vec<T, 8>(dh, d);
         } else {
-            const unsigned count = min(8u, cols - n);
-            const Vec<T, 8> a = load_any<T>(gate + m * ldg + n, count), b = load_any<T>(up + m * ldu + n, count), c = load_any<T>(dh + m * ldh + n, count);
+            const unsigned count = min(8u, a.cols - n);
+            const Vec<T, 8> x = load_any<T>(gate, count), y = load_any<T>(up, count), z = load_any<T>(dh, count);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = to_f32<T>(a.v[j]), u[j] = to_f32<T>(b.v[j]), d[j] = to_f32<T>(c.v[j]);
+            for (int j = 0; j < 8; ++j) g[j] = to_f32<T>(x.v[j]), u[j] = to_f32<T>(y.v[j]), d[j] = to_f32<T>(z.v[j]);
         }
-        ungate(act, g, u, d);
-        store_vec<T, 8>(dg + m * ld + n, g);
-        store_vec<T, 8>(du + m * ld + n, u);
+        ungate(a.act, g, u, d);
+        store_vec<T, 8>(static_cast<T*>(a.dg) + m * a.ld + n, g);
+        store_vec<T, 8>(static_cast<T*>(a.du) + m * a.ld + n, u);
     }
 }
 
 // dx from the parts of its sums, in their order
-template <class T, bool kWidePath>
-__global__ void __launch_bounds__(128) glu_add_parts_kernel(const float* __restrict__ sums, unsigned parts, unsigned m, unsigned n, unsigned ld, T* __restrict__ out,
-                                                            size_t ldo) {
-    grid_release();
-    grid_wait();
-    const unsigned c = (blockIdx.x * 128 + threadIdx.x) * 4, row = blockIdx.y;
-    if (c >= n) return;
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (unsigned k = 0; k < parts; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(sums + ((size_t)k * m + row) * ld + c);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-    }
-    const float v[4] = {s.x, s.y, s.z, s.w};
-    T* to = out + (size_t)row * ldo + c;
-    if (kWidePath && c + 4 <= n) {
-        store_vec<T, 4>(to, v);
-    } else {
+struct AddArgs {
+    const float* sums;
+    void* out;
+    size_t ldo;
+    unsigned parts, m, n, ld;   // no parts: nothing to add
+    bool wide;
+};
+template <class T>
+__device__ __forceinline__ void add_rows(const AddArgs& a) {
+    const unsigned c = (blockIdx.x * 128 + threadIdx.x) * 4;
+    if (c >= a.n) return;
+    for (unsigned row = blockIdx.y; row < a.m; row += gridDim.y) {
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (unsigned k = 0; k < a.parts; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(a.sums + ((size_t)k * a.m + row) * a.ld + c);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        T* to = static_cast<T*>(a.out) + (size_t)row * a.ldo + c;
+        if (a.wide && c + 4 <= a.n) {
+            store_vec<T, 4>(to, v);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < n) to[j] = from_f32<T>(v[j]);
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.n) to[j] = from_f32<T>(v[j]);
+        }
     }
 }
 
@@ -576,14 +591,23 @@ struct AlignArgs {
     void* to[3];
     size_t ld_to[3];
 };
+// What comes before the products, in one launch: the gradients of the projections (blockIdx.z 0, if asked for) and the operands.
 template <class T>
-__global__ void __launch_bounds__(128) glu_align_kernel(const __grid_constant__ AlignArgs a) {
-    const Operand& x = a.from[blockIdx.z];
-    const size_t c = (blockIdx.x * 128 + threadIdx.x) * 8, ld = a.ld_to[blockIdx.z];
+__global__ void __launch_bounds__(128) glu_before_kernel(const __grid_constant__ SplitArgs split, const __grid_constant__ AlignArgs a) {
+    unsigned z = blockIdx.z;
+    if (split.rows) {
+        if (z == 0) {
+            split_rows<T>(split);
+            return;
+        }
+        --z;
+    }
+    const Operand& x = a.from[z];
+    const size_t c = (blockIdx.x * 128 + threadIdx.x) * 8, ld = a.ld_to[z];
     if (c >= ld) return;
     for (size_t r = blockIdx.y; r < x.rows; r += gridDim.y) {
         const Vec<T, 8> v = load_any<T>(static_cast<const T*>(x.p) + r * x.ld + c, (unsigned)min((size_t)8, x.cols - c));
-        *reinterpret_cast<Vec<T, 8>*>(static_cast<T*>(a.to[blockIdx.z]) + r * ld + c) = v;
+        *reinterpret_cast<Vec<T, 8>*>(static_cast<T*>(a.to[z]) + r * ld + c) = v;
     }
 }
 
@@ -593,14 +617,19 @@ struct PlaceArgs {
     const void* from[3];
     void* to[3];
     size_t ld_from[3], ld_to[3];
-    unsigned rows, cols;
+    unsigned rows[3], cols[3], n;
 };
 template <class T>
-__global__ void __launch_bounds__(128) glu_place_kernel(const __grid_constant__ PlaceArgs a) {
-    const int g = blockIdx.x * 128 + threadIdx.x, cols = (int)a.cols;
-    for (size_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const T* from = static_cast<const T*>(a.from[blockIdx.z]) + r * a.ld_from[blockIdx.z];
-        T* to = static_cast<T*>(a.to[blockIdx.z]) + r * a.ld_to[blockIdx.z];
+__global__ void __launch_bounds__(128) glu_after_kernel(const __grid_constant__ PlaceArgs a, const __grid_constant__ AddArgs add) {
+    const unsigned z = blockIdx.z;
+    if (z == a.n) {
+        add_rows<T>(add);
+        return;
+    }
+    const int g = blockIdx.x * 128 + threadIdx.x, cols = (int)a.cols[z];
+    for (size_t r = blockIdx.y; r < a.rows[z]; r += gridDim.y) {
+        const T* from = static_cast<const T*>(a.from[z]) + r * a.ld_from[z];
+        T* to = static_cast<T*>(a.to[z]) + r * a.ld_to[z];
         const int e = g * 8 - (int)((reinterpret_cast<uintptr_t>(to) & 15) / 2);   // the granule's first value
         if (e >= cols) continue;
         if (e >= 0 && e + 8 <= cols) {
@@ -612,11 +641,14 @@ __global__ void __launch_bounds__(128) glu_place_kernel(const __grid_constant__ 
 }
 
 bool copyable(const void* p, size_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
-// Makes operands readable by tensor copies, those that are not through the workspace.
+// rows of a grid whose blocks take several each: as many as are resident at once (16 blocks of 128 threads to an SM), no more
+unsigned grid_rows(size_t rows, unsigned blocks_a_row) { return (unsigned)std::min<size_t>(rows, std::max(1u, 16u * sm_count() / blocks_a_row)); }
+// Makes operands readable by tensor copies, those that are not through the workspace, and splits the gradient where that is asked for.
 template <class T>
-int align(std::initializer_list<Operand*> operands, Scratch* scratch, cudaStream_t s) {
+int before(const SplitArgs& split, std::initializer_list<Operand*> operands, Scratch* scratch, cudaStream_t s) {
     AlignArgs a = {};
-    unsigned n = 0, rows = 0, blocks = 0;
+    unsigned n = 0, across = split.rows ? div_up(split.cols, 8 * 128) : 0;
+    size_t rows = split.rows;
     for (Operand* x : operands) {
         const size_t ld = (x->cols + 7) / 8 * 8;
         if (x->rows == 1) x->ld = ld;   // never used
@@ -625,12 +657,13 @@ int align(std::initializer_list<Operand*> operands, Scratch* scratch, cudaStream
         a.ld_to[n] = ld;
         if (!(a.to[n] = scratch->get_n<T>(x->rows * ld))) return ZKB_ERR_CUDA;
         x->p = a.to[n], x->ld = ld;
-        rows = std::max(rows, (unsigned)x->rows), blocks = std::max(blocks, div_up(ld, 8 * 128));
+        rows = std::max(rows, x->rows), across = std::max(across, div_up(ld, 8 * 128));
         ++n;
     }
+    n += split.rows != 0;
     if (!n) return ZKB_OK;
-    const auto glu_align = glu_align_kernel<T>;
-    ZKB_LAUNCH(glu_align, dim3(blocks, std::min(rows, std::max(1u, 32u * sm_count() / blocks)), n), 128, 0, s, a);
+    const auto glu_before = glu_before_kernel<T>;
+    ZKB_LAUNCH(glu_before, dim3(across, grid_rows(rows, across * n), n), 128, 0, s, split, a);
     return ZKB_OK;
 }
 
@@ -649,23 +682,25 @@ void lay_results(Results* r, size_t m, size_t n, unsigned tile_cols, size_t k) {
 }
 // Sets a result's place, or room for it in the workspace and a note of where it goes.
 template <class T>
-int set_result(Results* r, int i, void* out, size_t ld, Scratch* scratch, PlaceArgs* later, unsigned* n) {
+int set_result(Results* r, int i, void* out, size_t ld, Scratch* scratch, PlaceArgs* later) {
     r->out[i] = out, r->ld[i] = ld;
     if (!out || copyable(out, ld)) return ZKB_OK;
     r->ld[i] = (r->n + 7) / 8 * 8;
     if (!(r->out[i] = scratch->get_n<T>((size_t)r->m * r->ld[i]))) return ZKB_ERR_CUDA;
-    later->from[*n] = r->out[i], later->ld_from[*n] = r->ld[i];
-    later->to[*n] = out, later->ld_to[*n] = ld;
-    later->rows = r->m, later->cols = r->n;
-    ++*n;
+    const unsigned n = later->n++;
+    later->from[n] = r->out[i], later->ld_from[n] = r->ld[i];
+    later->to[n] = out, later->ld_to[n] = ld;
+    later->rows[n] = r->m, later->cols[n] = r->n;
     return ZKB_OK;
 }
 template <class T>
-int place_results(const PlaceArgs& a, unsigned n, cudaStream_t s) {
+int after(const PlaceArgs& a, const AddArgs& add, cudaStream_t s) {
+    unsigned across = add.parts ? div_up(add.n, 4 * 128) : 0, rows = add.parts ? add.m : 0;
+    for (unsigned i = 0; i < a.n; ++i) across = std::max(across, div_up(a.cols[i] + 7, 8 * 128)), rows = std::max(rows, a.rows[i]);
+    const unsigned n = a.n + (add.parts != 0);
     if (!n) return ZKB_OK;
-    const unsigned across = div_up(a.cols + 7, 8 * 128);
-    const auto glu_place = glu_place_kernel<T>;
-    ZKB_LAUNCH(glu_place, dim3(across, std::min(a.rows, std::max(1u, 32u * sm_count() / across)), n), 128, 0, s, a);
+    const auto glu_after = glu_after_kernel<T>;
+    ZKB_LAUNCH(glu_after, dim3(across, grid_rows(rows, across * n), n), 128, 0, s, a, add);
     return ZKB_OK;
 }
 
@@ -699,7 +734,7 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     }
     Scratch scratch(s);
     Operand x = {a.x, a.ldx, a.tokens, a.in}, wg = {a.wg, a.ldwg, a.in, a.hidden}, wu = {a.wu, a.ldwu, a.in, a.hidden};
-    ZKB_TRY(align<T>({&x, &wg, &wu}, &scratch, s));
+    ZKB_TRY(before<T>(SplitArgs{}, {&x, &wg, &wu}, &scratch, s));
     int* const flag = tc::wait_flag();
     if (!flag) return ZKB_ERR_CUDA;
     if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, flag, &scratch, s);
@@ -713,12 +748,11 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     ZKB_TRY(tc::make_map(&p.b[1], kCode<T>, wu.p, a.in, a.hidden, wu.ld, kDepth));
     lay_results(&p.r, a.tokens, a.hidden, kHalf, a.in);
     PlaceArgs later = {};
-    unsigned n = 0;
-    ZKB_TRY(set_result<T>(&p.r, 0, a.h, a.ldh, &scratch, &later, &n));
-    ZKB_TRY(set_result<T>(&p.r, 1, a.gate_out, a.ldg, &scratch, &later, &n));
-    ZKB_TRY(set_result<T>(&p.r, 2, a.up_out, a.ldu, &scratch, &later, &n));
+    ZKB_TRY(set_result<T>(&p.r, 0, a.h, a.ldh, &scratch, &later));
+    ZKB_TRY(set_result<T>(&p.r, 1, a.gate_out, a.ldg, &scratch, &later));
+    ZKB_TRY(set_result<T>(&p.r, 2, a.up_out, a.ldu, &scratch, &later));
     ZKB_TRY(product_launch<T>(p, (size_t)p.r.row_tiles * p.r.col_tiles, s));
-    return place_results<T>(later, n, s);
+    return after<T>(later, AddArgs{}, s);
 }
 
 template <class T>
@@ -735,18 +769,15 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     T* dg = scratch.get_n<T>(a.tokens * ld);
     T* du = scratch.get_n<T>(a.tokens * ld);
     if (!dg || !du) return ZKB_ERR_CUDA;
-    const auto glu_split = copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh) ? glu_split_kernel<T, true> : glu_split_kernel<T, false>;
-    const unsigned across = div_up(F, 8 * 128);
-    ZKB_LAUNCH(glu_split, dim3(across, (unsigned)std::min<size_t>(a.tokens, std::max(1u, 32u * sm_count() / across))), 128, 0, s,
-                          static_cast<const T*>(a.gate), a.ldg, static_cast<const T*>(a.up), a.ldu, static_cast<const T*>(a.dh), a.lddh, dg, du, ld,
-                          (unsigned)a.tokens, (unsigned)F, a.act);
+    const SplitArgs split = {a.gate, a.up, a.dh, dg, du, a.ldg, a.ldu, a.lddh, ld, (unsigned)a.tokens, (unsigned)F, a.act,
+                             copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh)};
     Operand x = {a.x, a.ldx, a.tokens, a.in}, wg = {a.wg, a.ldwg, a.in, F}, wu = {a.wu, a.ldwu, a.in, F};
-    if (a.dx && a.dwg) ZKB_TRY(align<T>({&x, &wg, &wu}, &scratch, s));
-    else if (a.dx) ZKB_TRY(align<T>({&wg, &wu}, &scratch, s));
-    else ZKB_TRY(align<T>({&x}, &scratch, s));
+    if (a.dx && a.dwg) ZKB_TRY(before<T>(split, {&x, &wg, &wu}, &scratch, s));
+    else if (a.dx) ZKB_TRY(before<T>(split, {&wg, &wu}, &scratch, s));
+    else ZKB_TRY(before<T>(split, {&x}, &scratch, s));
     GradArgs p = {};
-    PlaceArgs later_dx = {}, later_dw = {};
-    unsigned n_dx = 0, n_dw = 0;
+    PlaceArgs later = {};
+    AddArgs add = {};
     if (!(p.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
     if (a.dx) {
         ZKB_TRY(tc::make_map(&p.dg_rows[0], kCode<T>, dg, a.tokens, F, ld, kHalf));
@@ -760,8 +791,8 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         ZKB_TRY(tc::make_map(&p.dg_cols[0], kCode<T>, dg, a.tokens, F, ld, kDepth));
         ZKB_TRY(tc::make_map(&p.dg_cols[1], kCode<T>, du, a.tokens, F, ld, kDepth));
         lay_results(&p.dw, a.in, F, kTile, a.tokens);
-        ZKB_TRY(set_result<T>(&p.dw, 0, a.dwg, a.lddwg, &scratch, &later_dw, &n_dw));
-        ZKB_TRY(set_result<T>(&p.dw, 1, a.dwu, a.lddwu, &scratch, &later_dw, &n_dw));
+        ZKB_TRY(set_result<T>(&p.dw, 0, a.dwg, a.lddwg, &scratch, &later));
+        ZKB_TRY(set_result<T>(&p.dw, 1, a.dwu, a.lddwu, &scratch, &later));
     }
     // at least 8 slices to a part: fewer cost more in the sums' way through memory than they save
     const size_t whole = (size_t)p.dx.row_tiles * p.dx.col_tiles, most = sm_count() / 2;
@@ -770,8 +801,9 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
         p.sums_ld = (p.dx.n + 3) / 4 * 4;
         p.sums = scratch.get_n<float>((size_t)p.parts * p.dx.m * p.sums_ld);
         if (!p.sums) return ZKB_ERR_CUDA;
+        add = {p.sums, a.dx, a.lddx, p.parts, p.dx.m, p.dx.n, p.sums_ld, copyable(a.dx, a.lddx)};
     } else if (a.dx) {
-        ZKB_TRY(set_result<T>(&p.dx, 0, a.dx, a.lddx, &scratch, &later_dx, &n_dx));
+        ZKB_TRY(set_result<T>(&p.dx, 0, a.dx, a.lddx, &scratch, &later));
     }
     const size_t longs = whole * p.parts, shorts = 2 * (size_t)p.dw.row_tiles * p.dw.col_tiles;
     const size_t pairs = std::min(longs + shorts, most), spare = pairs - longs % pairs;
@@ -779,19 +811,13 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     const unsigned cost_long = std::max(16u, 2 * p.dx.slices / p.parts), cost_short = std::max(16u, p.dw.slices);
     if (shorts && longs % pairs) p.head = (unsigned)std::min<size_t>((cost_long + cost_short / 2) / cost_short, shorts / spare);
     ZKB_TRY(product_launch<T>(p, longs + shorts, s));
-    ZKB_TRY(place_results<T>(later_dx, n_dx, s));
-    ZKB_TRY(place_results<T>(later_dw, n_dw, s));
-    if (p.parts == 1) return ZKB_OK;
-    const auto glu_add_parts = copyable(a.dx, a.lddx) ? glu_add_parts_kernel<T, true> : glu_add_parts_kernel<T, false>;
-    ZKB_LAUNCH(glu_add_parts, dim3(div_up(p.dx.n, 4 * 128), p.dx.m), 128, 0, s, p.sums, p.parts, p.dx.m, p.dx.n, p.sums_ld, static_cast<T*>(a.dx), a.lddx);
-    return ZKB_OK;
+    return after<T>(later, add, s);
 }
 
 int check_matrix(const char* who, const char* name, const void* p, size_t rows, size_t cols, size_t ld, bool needed) {
-    const std::string w = std::string(who) + ": " + name;
-    if (!p) return needed ? fail(ZKB_ERR_ARG, w + " is missing") : ZKB_OK;
-    if (ld < cols && rows > 1) return fail(ZKB_ERR_DIM, w + ": row stride below the row's length");
-    return check_device(p, 2, w.c_str());
+    if (!p) return needed ? fail(ZKB_ERR_ARG, std::string(who) + ": " + name + " is missing") : ZKB_OK;
+    if (ld < cols && rows > 1) return fail(ZKB_ERR_DIM, std::string(who) + ": " + name + ": row stride below the row's length");
+    return check_device(p, 2, who, name);
 }
 int check_common(const char* who, int dtype, int act, const GluArgs& a) {
     const std::string w(who);

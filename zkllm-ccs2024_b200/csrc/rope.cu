@@ -191,8 +191,8 @@ int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, 
     if (tokens > 0x7fffffffull || batch > 0x7fffffffull || batch * tokens > 0x7fffffffull)
         return fail(ZKB_ERR_LIMIT, "zkb_rope: 2^31 tokens or more");
     if (!d_inv_freq) return fail(ZKB_ERR_ARG, "zkb_rope: no frequencies");
-    ZKB_TRY(check_device(d_inv_freq, 8, "zkb_rope: d_inv_freq"));
-    ZKB_TRY(check_device(d_positions, 8, "zkb_rope: d_positions"));
+    ZKB_TRY(check_device(d_inv_freq, 8, "zkb_rope", "d_inv_freq"));
+    ZKB_TRY(check_device(d_positions, 8, "zkb_rope", "d_positions"));
 
     RopeArgs a = {};
     const size_t es = type_size(dtype), v = 16 / es;
@@ -202,8 +202,8 @@ int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, 
         if (!h.heads) continue;
         if (!h.d_in || !h.d_out) return fail(ZKB_ERR_ARG, "zkb_rope: tensor without memory");
         if (h.heads > 65535) return fail(ZKB_ERR_LIMIT, "zkb_rope: more than 65535 heads");
-        ZKB_TRY(check_device(h.d_in, es, "zkb_rope: d_in"));
-        ZKB_TRY(check_device(h.d_out, es, "zkb_rope: d_out"));
+        ZKB_TRY(check_device(h.d_in, es, "zkb_rope", "d_in"));
+        ZKB_TRY(check_device(h.d_out, es, "zkb_rope", "d_out"));
         const bool same = h.d_in == h.d_out;
         if (same && (h.in_batch != h.out_batch || h.in_token != h.out_token || h.in_head != h.out_head))
             return fail(ZKB_ERR_ARG, "zkb_rope: in place with other strides");
