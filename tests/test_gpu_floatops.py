@@ -853,3 +853,28 @@ print("same")
 """.format(root=str(root))
     res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=root)
     assert res.returncode == 0 and "same" in res.stdout, res.stdout[-1000:] + res.stderr[-3000:]
+
+
+def test_the_rms_inv_stage_feeds_rmsnorm(tmp_path):
+    """the driver's rms-inv stage writes what the rmsnorm stage reads: within one unit of the formula in 64 bits (32-bit statistics of values of
+    2^16 are off by less than 2^-20 of themselves, a sixteenth of a unit, which moves a rounding now and then); then rmsnorm proves with it, in
+    one batch"""
+    import numpy as np
+    from tests.test_gpu_drivers import BIN, make_param, rescale, run, save_int
+    rng = np.random.Generator(np.random.PCG64(5))
+    seq, embed = 256, 256
+    x = np.rint(rng.standard_normal((seq, embed)) * 65536 * np.exp(rng.standard_normal((seq, 1)))).astype(np.int64)
+    w = np.rint((1.0 + 0.1 * rng.standard_normal(embed)) * 65536).astype(np.int64)
+    save_int(tmp_path / "x.bin", x)
+    make_param(BIN, tmp_path, "layer-0", "input_layernorm.weight", w, 1, embed, embed)
+    (tmp_path / "script").write_text(f"rms-inv x.bin {seq} {embed} 1e-5\nrmsnorm input x.bin {seq} {embed} {tmp_path} layer-0 out.bin\n")
+    run(BIN, "zkllm-driver", ["batch", "script"], tmp_path)
+    got = np.fromfile(tmp_path / "rms_inv_temp.bin", dtype=np.int32).astype(np.int64)
+    want = 65536.0 / np.sqrt(((x / 65536.0) ** 2).mean(axis=1) + 1e-5)
+    assert got.shape == (seq,) and np.abs(got - want).max() <= 0.5 + 2.0 ** -20 * want.max()
+    exp = rescale(rescale(np.outer(got, w), 1 << 16) * x, 1 << 16)
+    assert np.array_equal(np.fromfile(tmp_path / "out.bin", dtype=np.int32).astype(np.int64), exp.reshape(-1))
+    import subprocess
+    for bad in (["x.bin", seq, embed + 1, 1e-5], ["x.bin", seq, embed, 0.0]):
+        res = subprocess.run([str(BIN / "zkllm-driver"), "rms-inv", *map(str, bad)], cwd=tmp_path, capture_output=True, text=True, timeout=120)
+        assert res.returncode != 0

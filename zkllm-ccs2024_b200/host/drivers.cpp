@@ -9,7 +9,11 @@
 //   zkllm-driver self-attn <linear|attn> <in.bin> <seq> <embed> <workdir> <layer-prefix> <out.bin>
 //   zkllm-driver ffn <in.bin> <seq> <embed> <hidden> <workdir> <layer-prefix> <out.bin>
 //   zkllm-driver skip-connection <x.bin> <y.bin> <out.bin>
+//   zkllm-driver rms-inv <in.bin> <seq> <embed> <eps>   (no counterpart among the reference's drivers)
 //   zkllm-driver batch <script|->      (no counterpart in the reference)
+//
+// `rms-inv` writes rms_inv_temp.bin, round(2^16 / sqrt(mean x^2 + eps)) for each row of x = in / 2^16, which the rmsnorm stage
+// reads and which the reference's Python side computes (llama-rmsnorm.py:37-39): a batch needs no other process between stages.
 //
 // `batch` reads one stage command per line ("ffn in.bin 2048 4096 ..."; blank
 // lines and lines starting with # are skipped) and runs them in this one
@@ -32,6 +36,7 @@
 // Each stage computes its fixed-point outputs in the field, proves them and
 // throws if a verifier equation fails, printing the reference's progress lines.
 #include <chrono>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <fstream>
@@ -305,12 +310,42 @@ int run_skip(const Args& a) {
     return 0;
 }
 
+int run_rms_inv(const Args& a) {
+    const uint seq = std::stoi(a.at(1)), embed = std::stoi(a.at(2));
+    const float eps = std::stof(a.at(3));
+    FrTensor X = FrTensor::from_int_bin(a.at(0));
+    if (X.size != (size_t)seq * embed) throw std::runtime_error("rms-inv: " + a.at(0) + " does not hold seq x embed values");
+    const auto check = [](int rc) {
+        if (rc != ZKB_OK) throw std::runtime_error(zkb_last_error());
+    };
+    struct Device {
+        void* p = nullptr;
+        ~Device() { zkb_free_default_stream(p); }
+    } values, inverse;
+    check(zkb_malloc(&values.p, sizeof(float) * (size_t)X.size));
+    check(zkb_malloc(&inverse.p, sizeof(float) * (size_t)seq));
+    check(zkb_fr_to_i32(reinterpret_cast<const zkb_fr_t*>(X.gpu_data), static_cast<int32_t*>(values.p), X.size, nullptr));
+    std::vector<int32_t> ints(X.size);
+    check(zkb_memcpy_d2h(ints.data(), values.p, sizeof(int32_t) * ints.size(), nullptr));
+    std::vector<float> x(X.size), inv(seq);
+    for (size_t i = 0; i < x.size(); ++i) x[i] = (float)(ints[i] / 65536.0);
+    check(zkb_memcpy_h2d(values.p, x.data(), sizeof(float) * x.size(), nullptr));
+    check(zkb_block_norm(ZKB_F32, ZKB_F32, seq, embed, values.p, embed, nullptr, 0, 0, nullptr, ZKB_GATE_NONE, nullptr, 0, 1.0f, 1, nullptr, eps, nullptr, 0,
+                         nullptr, 0, nullptr, static_cast<float*>(inverse.p), nullptr));
+    check(zkb_memcpy_d2h(inv.data(), inverse.p, sizeof(float) * inv.size(), nullptr));
+    std::vector<int> fixed(seq);
+    for (uint i = 0; i < seq; ++i) fixed[i] = (int)std::lround(65536.0 * inv[i]);
+    FrTensor(seq, fixed.data()).save_int("rms_inv_temp.bin");
+    return 0;
+}
+
 typedef std::map<std::string, std::pair<std::function<int(const Args&)>, size_t>> StageTable;
 
 const StageTable& stage_table() {
     static const StageTable stages = {
         {"ppgen", {run_ppgen, 2}},         {"commit-param", {run_commit_param, 5}}, {"rmsnorm", {run_rmsnorm, 7}},
-        {"self-attn", {run_self_attn, 7}}, {"ffn", {run_ffn, 7}},                   {"skip-connection", {run_skip, 3}}};
+        {"self-attn", {run_self_attn, 7}}, {"ffn", {run_ffn, 7}},                   {"skip-connection", {run_skip, 3}},
+        {"rms-inv", {run_rms_inv, 4}}};
     return stages;
 }
 
@@ -387,7 +422,7 @@ int main(int argc, char* argv[]) {
     std::string stage = self;
     if (!stages.count(stage)) {
         if (argc < 2 || !stages.count(argv[1])) {
-            cerr << "usage: " << self << " <ppgen|commit-param|rmsnorm|self-attn|ffn|skip-connection|batch> <stage arguments>" << endl;
+            cerr << "usage: " << self << " <ppgen|commit-param|rmsnorm|self-attn|ffn|skip-connection|rms-inv|batch> <stage arguments>" << endl;
             return 2;
         }
         stage = argv[1];
