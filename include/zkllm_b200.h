@@ -333,6 +333,8 @@ int zkb_softmax_decompose(const zkb_fr_t* d_X, const uint32_t* h_bs, unsigned K,
  *  - Results do not depend on timing: the same call gives the same bits.
  *  - Calls are asynchronous on `stream`, may be captured into a graph, and take their workspace from the library's pool
  *    for each call, so that captured graphs share none.
+ *  - Waits inside these kernels end after two seconds; the next call then returns ZKB_ERR_CUDA and says that an earlier
+ *    one's results are incomplete.
  *  - An output may be the memory of an input of the same shape and strides where that is said; otherwise memory of
  *    outputs overlaps nothing. */
 #define ZKB_F32  0

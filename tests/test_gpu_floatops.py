@@ -878,3 +878,42 @@ def test_the_rms_inv_stage_feeds_rmsnorm(tmp_path):
     for bad in (["x.bin", seq, embed + 1, 1e-5], ["x.bin", seq, embed, 0.0]):
         res = subprocess.run([str(BIN / "zkllm-driver"), "rms-inv", *map(str, bad)], cwd=tmp_path, capture_output=True, text=True, timeout=120)
         assert res.returncode != 0
+
+
+def test_a_call_waits_for_the_one_before(zkb):
+    """each kind of call takes what the one before it on the stream has just written, many rows of it, with nothing between: norm to few tokens, few
+    tokens to norm, norm to norm, gradients of the norm to few tokens, few tokens to few tokens in the same workspace"""
+    t, n, e, f = torch.bfloat16, 6000, 1024, 1536
+    x, wg, wu, _, _, _ = glu_inputs(n, e, f, t, 3)
+    r, y, pg, gg, gv, dz, dr = norm_inputs(n, e, t, t, "channel", True, 3)
+    z1, z2, dx, dy = (torch.empty(n, e, device="cuda", dtype=t) for _ in range(4))
+    last = slice(n - 16, n)
+    h = [torch.empty(16, f, device="cuda", dtype=t) for _ in range(4)]
+    zh = torch.empty(16, f, device="cuda", dtype=t)
+    dg, dp, dw = torch.empty_like(gv), torch.empty_like(pg), torch.empty_like(gg)
+
+    def chain(pause):
+        for o in [z1, z2, dx, dy, zh, dg, dp, dw] + h:
+            o.zero_()
+        pause()
+        norm_call(zkb, 2, 2, x, None, False, None, "none", None, 1.0, gg, 1e-5, None, z1, None, None)
+        pause()
+        glu_call(zkb, 2, "silu", z1[last], wg, wu, h[0], None, None)
+        pause()
+        norm_call(zkb, 2, 2, h[0], None, False, None, "none", None, 1.0, None, 1e-5, None, zh, None, None)
+        pause()
+        norm_call(zkb, 2, 2, z1, y, True, pg, "channel", gv, 0.7, gg, 1e-5, None, z2, None, None)
+        pause()
+        glu_call(zkb, 2, "silu", z2[last], wg, wu, h[1], None, None)
+        pause()
+        glu_call(zkb, 2, "gelu", z1[last], wg, wu, h[2], None, None)
+        pause()
+        back_call(zkb, 2, 2, z2, y, True, pg, "channel", gv, 0.7, gg, 1e-5, dz, dr, dx, dy, dg, dp, dw)
+        pause()
+        glu_call(zkb, 2, "silu", dx[last], wg, wu, h[3], None, None)
+        torch.cuda.synchronize()
+        return [o.clone() for o in [z1, z2, dx, dy, zh, dg, dp, dw] + h]
+    want = chain(torch.cuda.synchronize)
+    for _ in range(20):
+        got = chain(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -72,6 +72,10 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 // the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 11 of both take their 128 rows of the other
 // accumulator out, so that a tile's epilogue runs beside the next tile's products.
 //
+// Measured: 2048 x 4096 x 11008 bf16, 238 to 299 us by the power the GPU has left (1.24 to 1.55 PFLOP/s; torch's two products alone 259 to
+// 265 us), the tensor pipe busy 87% of the time; gradients 595 us, 540 at best.  One block to a tile of 128 x 256 took 360 us; a switch over the
+// activation inside the epilogue's loop 337; the gradients' two kinds of tiles in a launch each 10% more.  Fetching slices ahead into L2 only cost.
+//
 // The forms of a tile:
 //   gated    first operand x; second the two weights side by side, 128 columns of each in a tile; result act(g) * u
 //   summed   dg, then du; w_gate, then w_up: one sum over both; result dx
@@ -330,6 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
 // narrow one, so that a slice in flight is nearly all weights.  The slices of all tiles, in order, are dealt out evenly: one
 // block per SM takes a run of them, whole tiles or parts of tiles, through one ring that never drains, and leaves the sums of each
 // (part of a) tile in the workspace; glu_few_finish_kernel adds the parts of a tile, in order, and applies the activation.
+// Measured: one token through 4096 x 11008 bf16, 34 us with both kernels (5.3 TB/s of 6.56; reading the same boxes and nothing else 29 us); 48
+// tokens through 5120 x 13824 f16, 56 us (5.0 TB/s).
 // Parts of a cluster that share a tile through distributed shared memory were measured before: no more than one such block ran on an
 // SM, and the ring of 72 KB that left to each read 4.0 TB/s.
 constexpr int kFewCols = 128, kFewThreads = 256;
@@ -373,6 +379,14 @@ __global__ void __launch_bounds__(kFewThreads) glu_few_kernel(const __grid_const
     const tc::Watch watch = {dead, p.flag};
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned total = p.tiles * p.slices, first = run_start(blockIdx.x, gridDim.x, total), last = run_start(blockIdx.x + 1, gridDim.x, total);
+    const auto fetch = [&](unsigned i) {   // the i-th slice of the run
+        const unsigned s = first + i, at = i % kR, col = s / p.slices * kFewCols, k = s % p.slices * kDepth;
+        const uint32_t a = tc::smem_address(ring) + at * kSlice, bar = full + 8 * at;
+        tc::barrier_expect(bar, kSlice);
+        for (int j = 0; j < kFewCols / 64; ++j) tc::load_box(&p.w[0], a + j * 8192, bar, col + j * 64, k);
+        for (int j = 0; j < kFewCols / 64; ++j) tc::load_box(&p.w[1], a + kA + j * 8192, bar, col + j * 64, k);
+        tc::load_box(&p.x, a + 2 * kA, bar, k, 0);
+    };
     if (threadIdx.x == 0) {
         for (int i = 0; i < kR; ++i) {
             tc::barrier_init(full + 8 * i, 1);
@@ -386,24 +400,23 @@ __global__ void __launch_bounds__(kFewThreads) glu_few_kernel(const __grid_const
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        grid_wait();
+        for (unsigned i = 0; i < kR && first + i < last; ++i) fetch(i);   // the first copies need nothing else of what is set up here
     }
     if (warp == 2) tc::tmem_alloc(tmem_at, 2 * kAcc);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(bars + 2 * kR + 6);
+    grid_release();
+    grid_wait();
 
     if (warp == 0 && lane == 0) {
-        unsigned issued = 0;
+        unsigned issued = min((unsigned)kR, last - first);
         bool fine = true;
-        for (unsigned s = first; s < last; ++s, ++issued) {
-            const unsigned at = issued % kR, col = s / p.slices * kFewCols, k = s % p.slices * kDepth;
-            if (!tc::barrier_wait(empty + 8 * at, ((issued / kR) & 1) ^ 1, watch)) { fine = false; break; }
-            const uint32_t a = tc::smem_address(ring) + at * kSlice, bar = full + 8 * at;
-            tc::barrier_expect(bar, kSlice);
-            for (int i = 0; i < kFewCols / 64; ++i) tc::load_box(&p.w[0], a + i * 8192, bar, col + i * 64, k);
-            for (int i = 0; i < kFewCols / 64; ++i) tc::load_box(&p.w[1], a + kA + i * 8192, bar, col + i * 64, k);
-            tc::load_box(&p.x, a + 2 * kA, bar, k, 0);
+        for (; first + issued < last; ++issued) {
+            if (!tc::barrier_wait(empty + 8 * (issued % kR), ((issued / kR) & 1) ^ 1, watch)) { fine = false; break; }
+            fetch(issued);
         }
         if (!fine)
             for (unsigned i = issued > kR ? issued - kR : 0; i < issued; ++i) tc::barrier_wait(full + 8 * (i % kR), (i / kR) & 1, watch, true);

@@ -106,9 +106,6 @@ __device__ __forceinline__ void barrier_arrive_in(uint32_t cluster_address) {
 // what lies outside reads as zero.  The address and ld * 2 have to be multiples of 16.
 int make_map(CUtensorMap* map, int dtype, const void* p, size_t rows, size_t cols, size_t ld, unsigned box_rows);
 
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
-}
 __device__ __forceinline__ void load_box(const CUtensorMap* m, uint32_t dst, uint32_t bar, int col, int row) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar),
