@@ -92,6 +92,10 @@ struct RowRing {
                                bars + 8 * slot);
             }
     }
+    // behind a kernel's last row: if a wait ran out, what is in flight lands before the block ends
+    __device__ __forceinline__ void close() const {
+        if (*watch.dead) tc::pause();
+    }
     __device__ __forceinline__ void wait(unsigned slot, uint32_t parity) const { tc::barrier_wait(bars + 8 * slot, parity, watch); }
     // in shared memory
     template <bool kAligned> __device__ __forceinline__ uint32_t row_of(int k, size_t row, unsigned slot) const {
@@ -387,6 +391,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_kernel(con
             store_group<T>(z_row, at, w);
         }
     }
+    ring.close();
 }
 
 // The gradients.  With p = dz w_pre, the gradient of r is d = dr + inv (p - r b), b = inv^2 mean(p r); with e = gate w_post, that of y
@@ -565,6 +570,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kBlocks) block_norm_backward_k
             }
         }
     }
+    ring.close();
     if (!a.partial) return;
     float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
