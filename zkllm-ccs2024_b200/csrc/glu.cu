@@ -335,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
 // block per SM takes a run of them, whole tiles or parts of tiles, through one ring that never drains, and leaves the sums of each
 // (part of a) tile in the workspace; glu_few_finish_kernel adds the parts of a tile, in order, and applies the activation.
 // Measured: one token through 4096 x 11008 bf16, 34 us with both kernels (5.3 TB/s of 6.56; reading the same boxes and nothing else 29 us); 48
-// tokens through 5120 x 13824 f16, 56 us (5.0 TB/s).
+// tokens through 5120 x 13824 f16, 55 us (5.2 TB/s).
 // Parts of a cluster that share a tile through distributed shared memory were measured before: no more than one such block ran on an
 // SM, and the ring of 72 KB that left to each read 4.0 TB/s.
 constexpr int kFewCols = 128, kFewThreads = 256;
@@ -478,27 +478,40 @@ __global__ void __launch_bounds__(kFewThreads) glu_few_kernel(const __grid_const
     }
 }
 
-// One block to 128 columns and a token.  Its blocks are launched while glu_few_kernel still runs and wait for its end.
-template <class T>
+// One block to 128 columns and kFewTogether tokens, whose parts are read together: four where there are more than that many tokens (48
+// tokens: 1 us less than one by one), else one (a single token: 0.2 us less than as one of four).  Its blocks are launched while
+// glu_few_kernel still runs and wait for its end.
+template <class T, unsigned kFewTogether>
 __global__ void __launch_bounds__(kFewCols) glu_few_finish_kernel(const __grid_constant__ FewEnd p) {
-    const unsigned tile = blockIdx.x, t = blockIdx.y, f = tile * kFewCols + threadIdx.x, total = p.tiles * p.slices;
+    const unsigned tile = blockIdx.x, t0 = blockIdx.y * kFewTogether, f = tile * kFewCols + threadIdx.x, total = p.tiles * p.slices;
     grid_release();
     grid_wait();
     const unsigned b0 = run_of(tile * p.slices, p.blocks, total), b1 = run_of(tile * p.slices + p.slices - 1, p.blocks, total);
     if (f >= p.hidden) return;
-    float g = 0.0f, u = 0.0f;
+    float g[kFewTogether] = {}, u[kFewTogether] = {};
     for (unsigned b = b0; b <= b1; ++b) {
-        const float* from = p.parts + ((size_t)(tile + b) * p.tokens + t) * 2 * kFewCols + threadIdx.x;
-        g += from[0];
-        u += from[kFewCols];
+        const float* from = p.parts + ((size_t)(tile + b) * p.tokens + t0) * 2 * kFewCols + threadIdx.x;
+#pragma unroll
+        for (unsigned i = 0; i < kFewTogether; ++i)
+            if (t0 + i < p.tokens) {
+                g[i] += from[i * 2 * kFewCols];
+                u[i] += from[i * 2 * kFewCols + kFewCols];
+            }
     }
-    if (p.out[1]) {
-        static_cast<T*>(p.out[1])[t * p.ld[1] + f] = from_f32<T>(g);
-        static_cast<T*>(p.out[2])[t * p.ld[2] + f] = from_f32<T>(u);
+    float h[kFewTogether];
+#pragma unroll
+    for (unsigned i = 0; i < kFewTogether; ++i) h[i] = g[i];
+    gate(p.act, h, u);
+#pragma unroll
+    for (unsigned i = 0; i < kFewTogether; ++i) {
+        const unsigned t = t0 + i;
+        if (t >= p.tokens) break;
+        if (p.out[1]) {
+            static_cast<T*>(p.out[1])[t * p.ld[1] + f] = from_f32<T>(g[i]);
+            static_cast<T*>(p.out[2])[t * p.ld[2] + f] = from_f32<T>(u[i]);
+        }
+        static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(h[i]);
     }
-    float h[1] = {g};
-    gate(p.act, h, {u});
-    static_cast<T*>(p.out[0])[t * p.ld[0] + f] = from_f32<T>(h[0]);
 }
 
 // 8 values from any address, of which `count` (1 to 8) belong to the row; the others come back as they may.  Reads whole 16-byte
@@ -734,8 +747,9 @@ int glu_few_launch(const GluArgs& a, Operand x, Operand wg, Operand wu, int* fla
     ZKB_CUDA(cudaFuncSetAttribute(glu_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     ZKB_TRY(launch_beside("glu_few", glu_few, blocks, kFewThreads, smem, s, p));
     const FewEnd e = {p.parts, p.tokens, (unsigned)a.hidden, p.tiles, p.slices, blocks, {a.h, a.gate_out, a.up_out}, {a.ldh, a.ldg, a.ldu}, a.act};
-    const auto glu_few_finish = glu_few_finish_kernel<T>;
-    return launch_beside("glu_few_finish", glu_few_finish, dim3(p.tiles, p.tokens), kFewCols, 0, s, e);
+    const unsigned together = p.tokens > 4 ? 4 : 1;
+    const auto glu_few_finish = together == 4 ? glu_few_finish_kernel<T, 4> : glu_few_finish_kernel<T, 1>;
+    return launch_beside("glu_few_finish", glu_few_finish, dim3(p.tiles, div_up(p.tokens, together)), kFewCols, 0, s, e);
 }
 
 template <class T>
