@@ -410,7 +410,9 @@ int zkb_glu(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidd
             void* d_up, size_t ldu, void* stream);
 /* Its gradients (no counterpart in the reference), from the two projections as zkb_glu kept them and the gradient of h:
  * d_dx [tokens, in_dim] (or NULL), d_dw_gate and d_dw_up [in_dim, hidden] (or both NULL).  The gradients of the projections are
- * rounded to the tensors' type before the products with the weights and with x. */
+ * rounded to the tensors' type before the products with the weights and with x, as the tensor cores take their operands: each is off by
+ * half a step.  In f16 that is done at a power-of-two scale that the call takes from their largest finite value, so that small
+ * and large ones keep their bits; one below 2^-29 of the largest is off by up to 2^-39 of the largest. */
 int zkb_glu_backward(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidden, const void* d_x, size_t ldx,
                      const void* d_w_gate, size_t ldwg, const void* d_w_up, size_t ldwu, const void* d_gate, size_t ldg,
                      const void* d_up, size_t ldu, const void* d_dh, size_t lddh, void* d_dx, size_t lddx, void* d_dw_gate,

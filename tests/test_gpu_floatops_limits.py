@@ -1,0 +1,82 @@
+"""GPU: the float operators of a layer where a type's range, a wait or a neighbouring call could spoil a result.
+
+Tolerances as in test_gpu_floatops.py: half a step of the type for each rounding, and for the 32-bit arithmetic before it what each test derives."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_floatops import (  # noqa: E402
+    ACTS, glu_back_call, glu_grads, glu_inputs, half_step, near, sum_slack, wide)
+
+
+# ---- gradients of the feed-forward block in f16 --------------------------------------------------------------------------------------------
+
+
+def check_scaled(act, x, wg, wu, gate, up, dh, dx, dwg, dwu, rows=slice(None)):
+    """The gradients of the projections are rounded to f16 at a scale that puts the call's largest at 2^14 or above: each is off by half a step of
+    its value or by 2^-25 at that scale, 2^-39 of the largest, and before that by 2^-19 of its factors' size (fast exponential)."""
+    t = torch.float16
+    dg, du, wx, wgg, wgu = glu_grads(act, x, wg, wu, gate, up, dh)
+    X, G, U, D, UP, GT = wide(x, wg, wu, dh, up, gate)
+    peak = torch.maximum(dg.abs().max(), du.abs().max())
+    eg = half_step(t) * dg.abs() + 2.0 ** -19 * (D * UP).abs() * (1 + GT.abs()) + 2.0 ** -39 * peak
+    eu = half_step(t) * du.abs() + 2.0 ** -20 * (D * GT).abs() + 2.0 ** -39 * peak
+    near(dx[rows], wx[rows], t, (eg @ G.abs().T + eu @ U.abs().T + sum_slack(2 * wg.shape[1]) * (dg.abs() @ G.abs().T + du.abs() @ U.abs().T))[rows])
+    if dwg is None:
+        return
+    near(dwg, wgg, t, X.abs().T @ eg + sum_slack(x.shape[0]) * (X.abs().T @ dg.abs()))
+    near(dwu, wgu, t, X.abs().T @ eu + sum_slack(x.shape[0]) * (X.abs().T @ du.abs()))
+    # the roundings are independent: relative to a result's norm they make half a step together, and the result's own another
+    for got, want in ((dx, wx), (dwg, wgg), (dwu, wgu)):
+        assert ((got.double() - want).norm() / want.norm()).item() <= 2.0 ** -10
+
+
+# sizes of dh, of up and gate, of x and of the weights: products far below f16's normal numbers and above its largest, results that f16 holds well
+@pytest.mark.parametrize("by", [(1e-5, 1.0, 64.0, 64.0), (1e-6, 1.0, 512.0, 1024.0), (2.0 ** -21, 0.05, 8192.0, 32768.0), (300.0, 300.0, 2.0 ** -9, 2.0 ** -8),
+                                (10000.0, 0.5, 2.0 ** -6, 2.0 ** -6)])
+@pytest.mark.parametrize("n,e,f,pad,shift", [(513, 72, 1032, 0, 0), (40, 264, 520, 5, 3), (777, 520, 136, 0, 0)])
+def test_glu_backward_f16_of_small_and_large_gradients(zkb, n, e, f, pad, shift, by):
+    for act in ACTS:
+        x, wg, wu, gate, up, dh = glu_inputs(n, e, f, torch.float16, n + e, pad, shift)
+        for m, k in ((dh, by[0]), (up, by[1]), (x, by[2]), (wg, by[3]), (wu, by[3])):
+            m.mul_(k)
+        if by[1] < 1:
+            gate.mul_(by[1])
+        dx, dwg, dwu = torch.full_like(x, math.nan), torch.full_like(wg, math.nan), torch.full_like(wu, math.nan)
+        glu_back_call(zkb, 1, act, x, wg, wu, gate, up, dh, dx, dwg, dwu)
+        check_scaled(act, x, wg, wu, gate, up, dh, dx, dwg, dwu)
+        again = [torch.empty_like(o) for o in (dx, dwg, dwu)]
+        glu_back_call(zkb, 1, act, x, wg, wu, gate, up, dh, *again)
+        assert all(torch.equal(a, b) for a, b in zip(again, (dx, dwg, dwu)))
+
+
+def test_glu_backward_f16_scale_follows_the_values(zkb):
+    """zeros give zeros; an infinity stays in its token and does not set the scale; a captured call replayed on other values takes their scale"""
+    n, e, f = 150, 72, 264
+    x, wg, wu, gate, up, dh = glu_inputs(n, e, f, torch.float16, 8)
+    x.mul_(64), wg.mul_(16), wu.mul_(16)
+    outs = [torch.full_like(x, math.nan), torch.full_like(wg, math.nan), torch.full_like(wu, math.nan)]
+    small = dh * 1e-5
+    live = torch.zeros_like(dh)
+    glu_back_call(zkb, 1, "silu", x, wg, wu, gate, up, live, *outs)
+    assert all((o == 0).all() for o in outs)
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        glu_back_call(zkb, 1, "silu", x, wg, wu, gate, up, live, *outs)
+    for values in (small, dh, small):
+        live.copy_(values)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_scaled("silu", x, wg, wu, gate, up, live, *outs)
+    bad = small.clone()
+    bad[7, 3], bad[9, 5] = math.inf, math.nan
+    glu_back_call(zkb, 1, "silu", x, wg, wu, gate, up, bad, *outs)
+    assert not outs[0][7].isfinite().any() and outs[0][9].isnan().all()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[[7, 9]] = False
+    small[[7, 9]] = 0
+    check_scaled("silu", x, wg, wu, gate, up, small, outs[0], None, None, keep)

@@ -110,6 +110,7 @@ struct GradArgs {
     unsigned head, parts;                    // parts: of dx's sums
     float* sums;                             // [parts][m][sums_ld], if there are several
     unsigned sums_ld;
+    const float* unscale;                    // f16: what the sums are multiplied by
     int* flag;
 };
 struct Tile { unsigned row, col, pair, part, from, to; bool paired; };   // from, to: its slices
@@ -274,6 +275,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
     } else if (warp >= 4) {
         char* stage = stages + (warp - 4) * kStageBytes;
         const unsigned side = (warp - 4) / 4;
+        constexpr bool kScaled = !kGated && std::is_same<T, __half>::value;
+        float unscale = 1.0f;
+        if constexpr (kScaled) unscale = *p.unscale;
         Tile t;
         for (unsigned i = 0; tile_of(p, i, first, step, &t); ++i) {
             const unsigned acc = i & 1;
@@ -299,6 +303,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
                 for (unsigned c = side * (kTile / 2); c < (side + 1) * (kTile / 2); c += 32) {
                     float v[32];
                     tc::load_columns(from + c, v);
+                    if constexpr (kScaled)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= unscale;
                     const unsigned col0 = t.col * kTile + c;
                     if (!t.paired && p.parts > 1) {   // this lane's row of a part, as it is
                         float* to = p.sums + ((size_t)t.part * r.m + row0 + lane) * p.sums_ld + col0;
@@ -537,7 +544,11 @@ __device__ __forceinline__ Vec<T, 8> load_any(const T* p, unsigned count) {
 
 // The gradients of the two projections' results.  They are rounded to the tensors' type, as the operands of the products that
 // follow have to be: each is off by half a step at most, independently, so a sum over them is off by no more, relative to its
-// norm, than its own rounding.
+// norm, than its own rounding.  bf16 has the range of the 32 bits that they are formed in.  f16 has not - gradients of 1e-6 would keep a
+// few bits, products above 65504 none - so there they are rounded at a scale, a power of two for the whole call that puts the largest of
+// them at 2^14 to 2^15, and the products' 32-bit sums are scaled back: a gradient is off by 2^-39 of the largest at most where
+// that is more than half its step (below 2^-29 of the largest).  The largest takes a pass of its own over the three inputs:
+// 42 us for 2048 x 11008, as long as the rounding pass, of 650 us for the whole call; 12 us for 777 x 2731 in unaligned rows.
 struct SplitArgs {
     const void *gate, *up, *dh;
     void *dg, *du;
@@ -545,26 +556,72 @@ struct SplitArgs {
     unsigned rows, cols;   // no rows: nothing to split
     int act;
     bool wide;
+    float *peaks, *unscale;   // f16: the largest value that each of n_peaks blocks has seen; where the scale's inverse goes
+    unsigned n_peaks;
 };
+// 8 values of both gradients from column n of row m on
+template <class T>
+__device__ __forceinline__ void split_values(const SplitArgs& a, unsigned m, unsigned n, float (&g)[8], float (&u)[8]) {
+    const T *gate = static_cast<const T*>(a.gate) + m * a.ldg + n, *up = static_cast<const T*>(a.up) + m * a.ldu + n,
+            *dh = static_cast<const T*>(a.dh) + m * a.ldh + n;
+    float d[8];
+    if (a.wide && n + 8 <= a.cols) {
+        load_vec<T, 8>(gate, g);
+        load_vec<T, 8>(up, u);
+        load_vec<T, 8>(dh, d);
+    } else {
+        const unsigned count = min(8u, a.cols - n);
+        const Vec<T, 8> x = load_any<T>(gate, count), y = load_any<T>(up, count), z = load_any<T>(dh, count);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = to_f32<T>(x.v[j]), u[j] = to_f32<T>(y.v[j]), d[j] = to_f32<T>(z.v[j]);
+    }
+    ungate(a.act, g, u, d);
+}
+// The largest of the values, none below zero, that the block's 128 threads hold; for every thread.
+__device__ __forceinline__ float block_peak(float peak) {
+    __shared__ unsigned part[4];
+    const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(peak));   // floats without a sign are ordered like their bits
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = most;
+    __syncthreads();
+    return __uint_as_float(max(max(part[0], part[1]), max(part[2], part[3])));
+}
+// Infinities and NaN have no part in the scale: they stay what they are under any.
+template <class T>
+__global__ void __launch_bounds__(128) glu_peak_kernel(const __grid_constant__ SplitArgs a) {
+    const unsigned n = (blockIdx.x * 128 + threadIdx.x) * 8;
+    float peak = 0.0f;
+    if (n < a.cols)
+        for (unsigned m = blockIdx.y; m < a.rows; m += gridDim.y) {
+            float g[8], u[8];
+            split_values<T>(a, m, n, g, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = fabsf(g[j]), y = fabsf(u[j]);
+                if (n + j < a.cols) peak = fmaxf(peak, fmaxf(isfinite(x) ? x : 0.0f, isfinite(y) ? y : 0.0f));
+            }
+        }
+    peak = block_peak(peak);
+    if (threadIdx.x == 0) a.peaks[blockIdx.y * gridDim.x + blockIdx.x] = peak;
+}
 template <class T>
 __device__ __forceinline__ void split_rows(const SplitArgs& a) {
+    float scale = 1.0f;
+    if constexpr (std::is_same<T, __half>::value) {
+        float peak = 0.0f;
+        for (unsigned i = threadIdx.x; i < a.n_peaks; i += 128) peak = fmaxf(peak, a.peaks[i]);
+        // 14 less the peak's exponent, -20 at least for products of f16 values; past 2^100 every result is zero in f16 anyway
+        const int up = min(100, 14 + 127 - (int)(__float_as_uint(block_peak(peak)) >> 23));
+        scale = __uint_as_float((unsigned)(127 + up) << 23);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.unscale = __uint_as_float((unsigned)(127 - up) << 23);
+    }
     const unsigned n = (blockIdx.x * 128 + threadIdx.x) * 8;
     if (n >= a.cols) return;
     for (unsigned m = blockIdx.y; m < a.rows; m += gridDim.y) {
-        const T *gate = static_cast<const T*>(a.gate) + m * a.ldg + n, *up = static_cast<const T*>(a.up) + m * a.ldu + n,
-                *dh = static_cast<const T*>(a.dh) + m * a.ldh + n;
-        float g[8], u[8], d[8];
-        if (a.wide && n + 8 <= a.cols) {
-            load_vec<T, 8>(gate, g);
-            load_vec<T, 8>(up, u);
-            load_vec<T, 8>(dh, d);
-        } else {
-            const unsigned count = min(8u, a.cols - n);
-            const Vec<T, 8> x = load_any<T>(gate, count), y = load_any<T>(up, count), z = load_any<T>(dh, count);
+        float g[8], u[8];
+        split_values<T>(a, m, n, g, u);
+        if constexpr (std::is_same<T, __half>::value)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = to_f32<T>(x.v[j]), u[j] = to_f32<T>(y.v[j]), d[j] = to_f32<T>(z.v[j]);
-        }
-        ungate(a.act, g, u, d);
+            for (int j = 0; j < 8; ++j) g[j] *= scale, u[j] *= scale;
         store_vec<T, 8>(static_cast<T*>(a.dg) + m * a.ld + n, g);
         store_vec<T, 8>(static_cast<T*>(a.du) + m * a.ld + n, u);
     }
@@ -793,16 +850,24 @@ int glu_backward_launch(const GluArgs& a, cudaStream_t s) {
     }
     if (!a.dx && !a.dwg) return ZKB_OK;
     Scratch scratch(s);
-    T* dg = scratch.get_n<T>(a.tokens * ld);
-    T* du = scratch.get_n<T>(a.tokens * ld);
-    if (!dg || !du) return ZKB_ERR_CUDA;
+    const dim3 peak_grid(div_up(F, 8 * 128), grid_rows(a.tokens, 2 * div_up(F, 8 * 128)));   // 8 blocks to an SM: fewer peaks to read again
+    const unsigned n_peaks = std::is_same<T, __half>::value ? peak_grid.x * peak_grid.y : 0;
+    T* const dg = scratch.get_n<T>(2 * a.tokens * ld + (n_peaks + 1) * sizeof(float) / sizeof(T));
+    if (!dg) return ZKB_ERR_CUDA;
+    T* const du = dg + a.tokens * ld;
+    float* const peaks = reinterpret_cast<float*>(du + a.tokens * ld);   // rows are whole 16 bytes
     const SplitArgs split = {a.gate, a.up, a.dh, dg, du, a.ldg, a.ldu, a.lddh, ld, (unsigned)a.tokens, (unsigned)F, a.act,
-                             copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh)};
+                             copyable(a.gate, a.ldg) && copyable(a.up, a.ldu) && copyable(a.dh, a.lddh), peaks, peaks + n_peaks, n_peaks};
+    if constexpr (std::is_same<T, __half>::value) {
+        const auto glu_peak = glu_peak_kernel<T>;
+        ZKB_LAUNCH(glu_peak, peak_grid, 128, 0, s, split);
+    }
     Operand x = {a.x, a.ldx, a.tokens, a.in}, wg = {a.wg, a.ldwg, a.in, F}, wu = {a.wu, a.ldwu, a.in, F};
     if (a.dx && a.dwg) ZKB_TRY(before<T>(split, {&x, &wg, &wu}, &scratch, s));
     else if (a.dx) ZKB_TRY(before<T>(split, {&wg, &wu}, &scratch, s));
     else ZKB_TRY(before<T>(split, {&x}, &scratch, s));
     GradArgs p = {};
+    p.unscale = split.unscale;
     PlaceArgs later = {};
     AddArgs add = {};
     if (!(p.flag = tc::wait_flag())) return ZKB_ERR_CUDA;
