@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from tests.test_gpu_floatops import (  # noqa: E402
-    ACTS, glu_back_call, glu_grads, glu_inputs, half_step, near, sum_slack, wide)
+    ACTS, TYPES, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, sum_slack, wide)
 
 
 # ---- gradients of the feed-forward block in f16 --------------------------------------------------------------------------------------------
@@ -80,3 +80,36 @@ def test_glu_backward_f16_scale_follows_the_values(zkb):
     keep[[7, 9]] = False
     small[[7, 9]] = 0
     check_scaled("silu", x, wg, wu, gate, up, small, outs[0], None, None, keep)
+
+
+# ---- the tail of the exact GELU ------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("n", (100, 300))
+def test_gelu_far_below_zero(zkb, kind, n):
+    """act(g) keeps its relative accuracy for gates from -8 to -3: the argument g / sqrt 2 is off by 2^-23 of itself, which moves erfc by g^2 = 64
+    times that, and erfcf by 4 steps of 2^-23: below 2^-16 together.  In the derivative the fast exponential of -g^2 / 2 is off by 41 steps of
+    2^-23 and its argument by 2^-23 of 32: below 2^-16 of each of its two terms."""
+    code, t = TYPES[kind]
+    f = 24
+    g = torch.linspace(-8, -3, n, device="cuda").to(t)[:, None]
+    one, zero = torch.ones(1, f, device="cuda", dtype=t), torch.zeros(1, f, device="cuda", dtype=t)
+    up = torch.full((1, f), 16384.0, device="cuda", dtype=t)
+    h, gate, u = (torch.empty(n, f, device="cuda", dtype=t) for _ in range(3))
+    glu_call(zkb, code, "gelu", g, one, up / g.abs().max(), h, gate, u)
+    assert torch.equal(gate, g.expand(n, f))
+    G = g.double()
+    cdf = 0.5 * torch.special.erfc(-G / math.sqrt(2))
+    prod = G * cdf * (G @ (up / g.abs().max()).double())
+    near(h, prod, t, 2.0 ** -16 * prod.abs())
+    pdf = torch.exp(-0.5 * G * G) / math.sqrt(2 * math.pi)
+    # one channel, so that dx is dg (weights 1 and 0) or du (0 and 1) itself
+    dh, ones, dx = torch.full((n, 1), 256.0, device="cuda", dtype=t), torch.ones(n, 1, device="cuda", dtype=t), torch.empty(n, 1, device="cuda", dtype=t)
+    glu_back_call(zkb, code, "gelu", ones, one[:, :1], zero[:, :1], g, ones, dh, dx, None, None)
+    want, size = 256 * (cdf + G * pdf), 256 * (cdf + G.abs() * pdf)
+    extra = 2.0 ** -39 * size.max() if kind == "f16" else 0.0
+    near(dx, want, t, half_step(t) * want.abs() + 2.0 ** -15 * size + extra)
+    glu_back_call(zkb, code, "gelu", ones, zero[:, :1], one[:, :1], g, ones, dh, dx, None, None)
+    want = 256 * G * cdf
+    near(dx, want, t, half_step(t) * want.abs() + 2.0 ** -16 * want.abs() + extra)

@@ -18,7 +18,7 @@ __device__ __forceinline__ float activate(float g, float* d) {
         if (kDerivative) *d = s * (1.0f + g * (1.0f - s));
         return g * s;
     } else if constexpr (kAct == ZKB_ACT_GELU) {
-        const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        const float c = 0.5f * erfcf(g * -0.70710678118654752f);   // 1 + erf would cancel below zero
         if (kDerivative) *d = c + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
         return g * c;
     } else if constexpr (kAct == ZKB_ACT_GELU_TANH) {
