@@ -2,6 +2,7 @@
 
 Tolerances as in test_gpu_floatops.py: half a step of the type for each rounding, and for the 32-bit arithmetic before it what each test derives."""
 import math
+import threading
 
 import pytest
 
@@ -9,7 +10,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from tests.test_gpu_floatops import (  # noqa: E402
-    ACTS, TYPES, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, sum_slack, wide)
+    ACTS, TYPES, back_call, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, norm_call, norm_inputs, sum_slack, wide)
 
 
 # ---- gradients of the feed-forward block in f16 --------------------------------------------------------------------------------------------
@@ -113,3 +114,63 @@ def test_gelu_far_below_zero(zkb, kind, n):
     glu_back_call(zkb, code, "gelu", ones, zero[:, :1], one[:, :1], g, ones, dh, dx, None, None)
     want = 256 * G * cdf
     near(dx, want, t, half_step(t) * want.abs() + 2.0 ** -16 * want.abs() + extra)
+
+
+# ---- calls beside one another ----------------------------------------------------------------------------------------------------------------------
+
+
+def widths(z, t, code, cols, seed):
+    r, y, pg, wg, gv, dz, dr = norm_inputs(40, cols, t, t, "channel", True, seed)
+    outs = [torch.zeros_like(r), torch.zeros_like(r), torch.zeros_like(gv), torch.zeros_like(pg), torch.zeros_like(wg), torch.zeros_like(r), torch.zeros_like(r)]
+
+    def go(st=None):
+        norm_call(z, code, code, r, y, True, pg, "channel", gv, 0.7, wg, 1e-5, outs[5], outs[6], None, None, st=st)
+        back_call(z, code, code, r, y, True, pg, "channel", gv, 0.7, wg, 1e-5, dz, dr, *outs[:5], st=st)
+    return go, outs
+
+
+def test_norms_of_different_widths_from_two_threads(zkb):
+    """narrow and wide rows run the same kernel with rings of different sizes: neither call's launch depends on the other's"""
+    made = [widths(zkb, torch.bfloat16, 2, cols, cols) for cols in (64, 2560)] + [widths(zkb, torch.float32, 0, cols, cols) for cols in (96, 2048)]
+    for go, _ in made:
+        go()
+    torch.cuda.synchronize()
+    want = [[o.clone() for o in outs] for _, outs in made]
+    streams, errors = [torch.cuda.Stream() for _ in made], []
+
+    def work(go, st):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(400):
+                go(st.cuda_stream)
+            st.synchronize()
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(go, st)) for (go, _), st in zip(made, streams)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for (_, outs), w in zip(made, want) for a, b in zip(outs, w))
+
+
+def test_norms_of_different_widths_in_one_graph(zkb):
+    made = [widths(zkb, torch.bfloat16, 2, cols, cols) for cols in (2560, 64, 2048, 128)]
+    for go, _ in made:
+        go()
+    torch.cuda.synchronize()
+    want = [[o.clone() for o in outs] for _, outs in made]
+    for _, outs in made:
+        for o in outs:
+            o.zero_()
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        for go, _ in made:
+            go()
+    widths(zkb, torch.bfloat16, 2, 8, 1)[0]()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for (_, outs), w in zip(made, want) for a, b in zip(outs, w))

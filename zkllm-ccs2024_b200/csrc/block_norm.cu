@@ -643,8 +643,9 @@ template <class Args> size_t lay_slot(Args* a, int matrices, size_t es) {
     a->slot_bytes = (unsigned)slot;
     return std::max<size_t>(slot, 16);
 }
-// slots of each block's ring; of its share, 1 KB is the system's and up to 3 KB the sums'
-size_t slots_for(size_t slot, int blocks_per_sm) { return std::min<size_t>(8, (224 * 1024 / blocks_per_sm - 4096 - kRingHead) / slot); }
+// The most that a block may ask for beside its sums when there are that many on an SM; of its share, 1 KB is the system's and up to 3 KB the sums'.
+constexpr size_t ring_share(int blocks_per_sm) { return 224 * 1024 / blocks_per_sm - 4096; }
+size_t slots_for(size_t slot, int blocks_per_sm) { return std::min<size_t>(8, (ring_share(blocks_per_sm) - kRingHead) / slot); }
 
 // The grid of a kernel over rows, and its ring: as many blocks as are resident, each with as many slots as fit.
 template <class L, class Kernel, class Args>
@@ -658,7 +659,9 @@ int plan_rows(Kernel kernel, unsigned threads, Args* a, unsigned* blocks, size_t
         while (resident > 1 && slots_for(slot, resident) < 3) --resident;
         a->slots = (unsigned)slots_for(slot, resident);
         *smem += a->slots * slot;
-        ZKB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)*smem));
+        // The limit belongs to the kernel, which calls of other widths run too, perhaps from another thread between this line and the
+        // launch: it is always the most that any of them asks for, never this call's size.
+        ZKB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_share(1)));
     }
     *blocks = (unsigned)std::min<size_t>(a->rows, (size_t)resident * sm_count());
     return ZKB_OK;
