@@ -1,6 +1,7 @@
 """GPU: the float operators of a layer where a type's range, a wait or a neighbouring call could spoil a result.
 
 Tolerances as in test_gpu_floatops.py: half a step of the type for each rounding, and for the 32-bit arithmetic before it what each test derives."""
+import ctypes
 import math
 import threading
 
@@ -10,7 +11,8 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from tests.test_gpu_floatops import (  # noqa: E402
-    ACTS, TYPES, back_call, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, norm_call, norm_inputs, sum_slack, wide)
+    ACTS, TYPES, back_call, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, norm_call, norm_inputs, rope_call, rope_freq, sum_slack,
+    wide)
 
 
 # ---- gradients of the feed-forward block in f16 --------------------------------------------------------------------------------------------
@@ -174,3 +176,19 @@ def test_norms_of_different_widths_in_one_graph(zkb):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for (_, outs), w in zip(made, want) for a, b in zip(outs, w))
+
+
+# ---- a call that failed ------------------------------------------------------------------------------------------------------------------------------
+
+
+def test_a_call_that_failed_leaves_the_next_one_alone(zkb):
+    """an allocation that cannot be met is that call's error, and not the next launch's"""
+    q = torch.randn(1, 5, 2, 64, device="cuda")
+    out, again, freq = torch.zeros_like(q), torch.zeros_like(q), rope_freq(64)
+    rope_call(zkb, 0, [(q, out)], 1, 5, 64, 64, False, freq, 1.0, None, 0, 5, False)
+    p = ctypes.c_void_p()
+    with pytest.raises(zkb.ZkbError):
+        zkb.call("zkb_malloc", ctypes.byref(p), ctypes.c_size_t(1 << 46))
+    rope_call(zkb, 0, [(q, again)], 1, 5, 64, 64, False, freq, 1.0, None, 0, 5, False)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)

@@ -26,6 +26,7 @@ int fail(int code, const std::string& msg) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();   // reported here: it is no business of the next call's launch check
     g_last_error = std::string(what) + ": " + cudaGetErrorString(e);
     return ZKB_ERR_CUDA;
 }
