@@ -192,3 +192,24 @@ def test_a_call_that_failed_leaves_the_next_one_alone(zkb):
     rope_call(zkb, 0, [(q, again)], 1, 5, 64, 64, False, freq, 1.0, None, 0, 5, False)
     torch.cuda.synchronize()
     assert torch.equal(out, again)
+
+
+# ---- the side input of the rmsnorm stage ----------------------------------------------------------------------------------------------------------------
+
+
+def test_rms_inv_refuses_what_its_file_cannot_hold(tmp_path):
+    """a row of zeros with a tiny eps has an inverse beyond 32 bits: the stage ends with an error and writes nothing; at the border it is exact"""
+    import subprocess
+
+    import numpy as np
+    from tests.test_gpu_drivers import BIN, save_int
+    x = np.ones((4, 8), dtype=np.int64) * 65536
+    x[2] = 0
+    save_int(tmp_path / "x.bin", x)
+    out = tmp_path / "rms_inv_temp.bin"
+    for eps, fits in ((1e-10, False), (1e-30, False), (4e-9, True)):
+        res = subprocess.run([str(BIN / "zkllm-driver"), "rms-inv", "x.bin", "4", "8", str(eps)], cwd=tmp_path, capture_output=True, text=True, timeout=120)
+        assert (res.returncode == 0) == fits and out.exists() == fits, res.stderr
+    got = np.fromfile(out, dtype=np.int32).astype(np.float64)
+    want = 65536.0 / np.sqrt(((x / 65536.0) ** 2).mean(axis=1) + np.float64(np.float32(4e-9)))
+    assert np.abs(got - want).max() <= 0.5 + 2.0 ** -20 * want.max()

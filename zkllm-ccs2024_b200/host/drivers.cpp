@@ -334,7 +334,11 @@ int run_rms_inv(const Args& a) {
                          nullptr, 0, nullptr, static_cast<float*>(inverse.p), nullptr));
     check(zkb_memcpy_d2h(inv.data(), inverse.p, sizeof(float) * inv.size(), nullptr));
     std::vector<int> fixed(seq);
-    for (uint i = 0; i < seq; ++i) fixed[i] = (int)std::lround(65536.0 * inv[i]);
+    for (uint i = 0; i < seq; ++i) {
+        const double value = 65536.0 * inv[i];
+        if (!(value < 2147483647.5)) throw std::runtime_error("rms-inv: row " + std::to_string(i) + " of " + a.at(0) + ": its inverse passes 32 bits, eps is too small");
+        fixed[i] = (int)std::lround(value);
+    }
     FrTensor(seq, fixed.data()).save_int("rms_inv_temp.bin");
     return 0;
 }
