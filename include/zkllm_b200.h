@@ -333,13 +333,19 @@ int zkb_softmax_decompose(const zkb_fr_t* d_X, const uint32_t* h_bs, unsigned K,
  *  - Results do not depend on timing: the same call gives the same bits.
  *  - Calls are asynchronous on `stream`, may be captured into a graph, and take their workspace from the library's pool
  *    for each call, so that captured graphs share none.
- *  - Waits inside these kernels end after two seconds; the next call then returns ZKB_ERR_CUDA and says that an earlier
- *    one's results are incomplete.
+ *  - Waits on a barrier inside these kernels end after two seconds, and the results of the call that waited are incomplete.  From then on
+ *    every call of these operators, zkb_sync and zkb_memcpy_d2h return ZKB_ERR_CUDA, on every thread and stream, until
+ *    zkb_wait_status resets it.  A host that waits by other means (an event, a framework's own synchronisation, a replayed graph)
+ *    asks zkb_wait_status afterwards.
  *  - An output may be the memory of an input of the same shape and strides where that is said; otherwise memory of
  *    outputs overlaps nothing. */
 #define ZKB_F32  0
 #define ZKB_F16  1
 #define ZKB_BF16 2
+
+/* ZKB_ERR_CUDA if a wait of these operators has run out in this process since the last reset, else ZKB_OK; reset != 0 makes it ZKB_OK from
+ * then on (no counterpart in the reference).  It waits for nothing itself: it speaks of the work that the host has waited for. */
+int zkb_wait_status(int reset);
 
 /* Rotary positions (no counterpart in the reference's C++).  Pair i of a head at position p is turned by the angle
  * p * inv_freq[i] and multiplied by `magnitude`;

@@ -11,8 +11,8 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from tests.test_gpu_floatops import (  # noqa: E402
-    ACTS, TYPES, back_call, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, norm_call, norm_inputs, rope_call, rope_freq, sum_slack,
-    wide)
+    ACTS, TYPES, back_call, glu_back_call, glu_call, glu_grads, glu_inputs, half_step, near, norm_call, norm_inputs, rope_call, rope_freq, stream,
+    sum_slack, wide)
 
 
 # ---- gradients of the feed-forward block in f16 --------------------------------------------------------------------------------------------
@@ -192,6 +192,116 @@ def test_a_call_that_failed_leaves_the_next_one_alone(zkb):
     rope_call(zkb, 0, [(q, again)], 1, 5, 64, 64, False, freq, 1.0, None, 0, 5, False)
     torch.cuda.synchronize()
     assert torch.equal(out, again)
+
+
+# ---- waits that ran out -----------------------------------------------------------------------------------------------------------------------------------
+
+
+def wait_word(zkb):
+    """the word that kernels raise, in host memory"""
+    where = getattr(zkb.lib(), "_ZN3zkb2tc9wait_flagEv")
+    where.restype = ctypes.POINTER(ctypes.c_int)
+    return where().contents
+
+
+def test_a_wait_that_ran_out_is_told_to_everyone(zkb):
+    """the word raised by the host, as a kernel would: each call and each wait of the library, on each thread, says so until it is reset; none runs"""
+    z = zkb
+    q = torch.randn(1, 5, 2, 64, device="cuda")
+    out, freq = torch.full_like(q, 3.0), rope_freq(64)
+    x, wg, wu, gate, up, dh = glu_inputs(9, 16, 24, torch.bfloat16, 1)
+    h = torch.full((9, 24), 3.0, device="cuda", dtype=torch.bfloat16)
+    r, y, pg, gg, gv, dz, dr = norm_inputs(4, 64, torch.float32, torch.float32, "none", True, 1)
+    zed = torch.full_like(r, 3.0)
+    host = torch.zeros(4)
+    word = wait_word(z)
+    assert z.call("zkb_wait_status", 0) == 0 and z.call("zkb_wait_status", 1) == 0
+    calls = [lambda: rope_call(z, 0, [(q, out)], 1, 5, 64, 64, False, freq, 1.0, None, 0, 5, False),
+             lambda: glu_call(z, 2, "silu", x, wg, wu, h, None, None),
+             lambda: glu_back_call(z, 2, "silu", x, wg, wu, gate, up, dh, h, None, None),
+             lambda: norm_call(z, 0, 0, r, None, False, None, "none", None, 1.0, None, 1e-5, None, zed, None, None),
+             lambda: back_call(z, 0, 0, r, y, True, pg, "none", None, 1.0, gg, 1e-5, dz, dr, zed, None, None, None, None),
+             lambda: z.call("zkb_sync", z._p(stream())),
+             lambda: z.call("zkb_memcpy_d2h", z._p(host.data_ptr()), z._p(q.data_ptr()), z.sz(16), z._p(stream())),
+             lambda: z.call("zkb_wait_status", 0)]
+    told = []
+
+    def everything():
+        for c in calls:
+            try:
+                c()
+                told.append("nothing")
+            except z.ZkbError as e:
+                told.append(e.code if "ran out" in e.msg else e.msg)
+    word.value = 1
+    try:
+        everything()
+        other = threading.Thread(target=everything)
+        other.start()
+        other.join()
+        assert told == [z.ERR_CUDA] * 2 * len(calls), told
+        torch.cuda.synchronize()
+        assert all((v == 3).all() for v in (out, h, zed))
+        with pytest.raises(z.ZkbError):
+            z.call("zkb_wait_status", 1)
+    finally:
+        word.value = 0
+    for c in calls:
+        c()
+
+
+def test_a_wait_that_nothing_ends(zkb, tmp_path):
+    """a block waits on barriers that nobody arrives at, by one thread and by a warp: both waits end, the kernel does, and the library says so"""
+    import os
+    import shutil
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("needs nvcc")
+    source = tmp_path / "wait.cu"
+    source.write_text("""
+#include "tensorcore.cuh"
+#include <cstdio>
+using namespace zkb;
+__global__ void lonely(int* flag, int* ended, bool by_warp) {
+    __shared__ uint64_t bar;
+    __shared__ int dead;
+    const uint32_t at = tc::smem_address(&bar);
+    if (threadIdx.x == 0) {
+        tc::barrier_init(at, 1);
+        dead = 0;
+    }
+    __syncthreads();
+    const tc::Watch watch = {&dead, flag};
+    bool fine = true;
+    if (by_warp) fine = tc::barrier_wait_warp(at, 0, watch);
+    else if (threadIdx.x == 0) fine = tc::barrier_wait(at, 0, watch);
+    if (threadIdx.x == 0) *ended = !fine && dead;
+}
+int main() {
+    int* const flag = tc::wait_flag();
+    int *ended, said[6], n = 0;
+    if (!flag || cudaMalloc(&ended, 8) != cudaSuccess || cudaMemset(ended, 0, 8) != cudaSuccess) return 1;
+    for (int w = 0; w < 2; ++w) {
+        said[n++] = zkb_wait_status(0);
+        lonely<<<1, 32>>>(flag, ended + w, w == 1);
+        said[n++] = zkb_sync(nullptr);
+        said[n++] = zkb_wait_status(1);
+    }
+    int got[2];
+    if (zkb_memcpy_d2h(got, ended, 8, nullptr) != ZKB_OK) return 2;
+    printf("%d %d | %d %d %d %d %d %d\\n", got[0], got[1], said[0], said[1], said[2], said[3], said[4], said[5]);
+    return 0;
+}
+""")
+    lib = root / "zkllm-ccs2024_b200" / "lib"
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-I", str(root / "zkllm-ccs2024_b200" / "csrc"), str(source), "-o", str(tmp_path / "wait"),
+                    "-L", str(lib), "-lzkllm_b200", "-Xlinker", f"-rpath={lib}"], check=True, timeout=300)
+    res = subprocess.run([str(tmp_path / "wait")], capture_output=True, text=True, timeout=60)
+    e = zkb.ERR_CUDA
+    assert res.returncode == 0 and res.stdout.strip() == f"1 1 | 0 {e} {e} 0 {e} {e}", res.stdout + res.stderr
 
 
 # ---- the side input of the rmsnorm stage ----------------------------------------------------------------------------------------------------------------

@@ -52,6 +52,7 @@ def lib() -> ctypes.CDLL:
 _CTYPES = {"p": ctypes.c_void_p, "n": ctypes.c_size_t, "i": ctypes.c_int, "u": ctypes.c_uint, "l": ctypes.c_int64, "f": ctypes.c_float,
            "d": ctypes.c_double}
 _FLOAT_OPERATORS = {
+    "zkb_wait_status": "i",
     "zkb_rope_frequencies": "i u d d d d d p p",
     "zkb_rope": "i p u n n n n i p f p l l i p",
     "zkb_block_norm": "i i n n p n p n i p i p n f i p f p n p n p p p",

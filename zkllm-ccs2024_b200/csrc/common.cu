@@ -423,7 +423,7 @@ int zkb_memcpy_h2d(void* d_dst, const void* h_src, size_t bytes, void* stream) {
 int zkb_memcpy_d2h(void* h_dst, const void* d_src, size_t bytes, void* stream) {
     ZKB_CUDA(cudaMemcpyAsync(h_dst, d_src, bytes, cudaMemcpyDeviceToHost, as_stream(stream)));
     ZKB_CUDA(cudaStreamSynchronize(as_stream(stream)));
-    return ZKB_OK;
+    return tc::check_wait_flag("zkb_memcpy_d2h");
 }
 int zkb_memcpy_d2d(void* d_dst, const void* d_src, size_t bytes, void* stream) {
     ZKB_CUDA(cudaMemcpyAsync(d_dst, d_src, bytes, cudaMemcpyDeviceToDevice, as_stream(stream)));
@@ -435,7 +435,7 @@ int zkb_memset0(void* d_dst, size_t bytes, void* stream) {
 }
 int zkb_sync(void* stream) {
     ZKB_CUDA(cudaStreamSynchronize(as_stream(stream)));
-    return ZKB_OK;
+    return tc::check_wait_flag("zkb_sync");
 }
 
 }  // extern "C"

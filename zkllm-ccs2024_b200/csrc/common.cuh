@@ -82,6 +82,12 @@ private:
     cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
 };
 
+namespace tc {
+// An error from the moment a wait in a kernel of this process ran out until zkb_wait_status resets it.  It is nobody's alone: the host
+// cannot tell whose results are incomplete, so no call, whichever thread or stream it is on, takes the news from the others.
+int check_wait_flag(const char* who);
+}  // namespace tc
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

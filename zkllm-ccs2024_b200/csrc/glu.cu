@@ -924,12 +924,13 @@ int check_common(const char* who, int dtype, int act, const GluArgs& a) {
 
 namespace tc {
 
-static int* g_wait_flag = nullptr;
-static std::mutex g_wait_mutex;
+static std::atomic<int*> g_wait_flag{nullptr};
 
 int* wait_flag() {
-    std::lock_guard<std::mutex> lock(g_wait_mutex);
-    if (!g_wait_flag) {
+    static std::mutex mutex;
+    if (int* made = g_wait_flag.load()) return made;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!g_wait_flag.load()) {
         const SetupDuringCapture setup;
         void* p = nullptr;
         const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
@@ -938,16 +939,14 @@ int* wait_flag() {
             return nullptr;
         }
         *static_cast<volatile int*>(p) = 0;
-        g_wait_flag = static_cast<int*>(p);
+        g_wait_flag.store(static_cast<int*>(p));
     }
-    return g_wait_flag;
+    return g_wait_flag.load();
 }
 int check_wait_flag(const char* who) {
-    std::lock_guard<std::mutex> lock(g_wait_mutex);
-    volatile int* f = g_wait_flag;
+    const volatile int* const f = g_wait_flag.load();
     if (!f || !*f) return ZKB_OK;
-    *f = 0;
-    return fail(ZKB_ERR_CUDA, std::string(who) + ": a wait of an earlier call ran out, its results are incomplete");
+    return fail(ZKB_ERR_CUDA, std::string(who) + ": a wait of an earlier call of the float operators ran out, its results are incomplete (zkb_wait_status resets this)");
 }
 
 int make_map(CUtensorMap* map, int dtype, const void* p, size_t rows, size_t cols, size_t ld, unsigned box_rows) {
@@ -974,6 +973,12 @@ int make_map(CUtensorMap* map, int dtype, const void* p, size_t rows, size_t col
 using namespace zkb;
 
 extern "C" {
+
+int zkb_wait_status(int reset) {
+    const int rc = tc::check_wait_flag("zkb_wait_status");
+    if (rc != ZKB_OK && reset) *static_cast<volatile int*>(tc::wait_flag()) = 0;
+    return rc;
+}
 
 int zkb_glu(int dtype, int activation, size_t tokens, size_t in_dim, size_t hidden, const void* d_x, size_t ldx, const void* d_w_gate, size_t ldwg,
             const void* d_w_up, size_t ldwu, void* d_h, size_t ldh, void* d_gate, size_t ldg, void* d_up, size_t ldu, void* stream) {

@@ -190,6 +190,7 @@ int zkb_rope(int dtype, const zkb_rope_tensor_t* h_tensors, unsigned n_tensors, 
     if (!rotary_dim || rotary_dim % 2 || rotary_dim > head_dim)
         return fail(ZKB_ERR_DIM, "zkb_rope: rotary_dim has to be even, positive and at most head_dim");
     if (head_dim > 8192) return fail(ZKB_ERR_LIMIT, "zkb_rope: head_dim above 8192");
+    ZKB_TRY(tc::check_wait_flag("zkb_rope"));
     if (!n_tensors || !batch || !tokens) return ZKB_OK;
     if (tokens > 0x7fffffffull || batch > 0x7fffffffull || batch * tokens > 0x7fffffffull)
         return fail(ZKB_ERR_LIMIT, "zkb_rope: 2^31 tokens or more");

@@ -36,8 +36,8 @@ __device__ __forceinline__ unsigned long long now_ns() {
     return t;
 }
 
-// No wait is endless: one that has lasted two seconds (or 2^28 tries) marks the block, and through `flag`, which the host reads at
-// the next call, the process; every role of the block then leaves its loop.
+// No wait on a barrier is endless: one that has lasted two seconds (or 2^28 tries) marks the block, and through `flag`, which the host
+// reads at every call and whenever it has waited for a stream, the process; every role of the block then leaves its loop.
 struct Watch {
     volatile int* dead;   // shared memory, of the block
     int* flag;            // mapped host memory
@@ -79,8 +79,6 @@ __device__ __forceinline__ void pause() {
 }
 // The flag that the kernels of this process raise (device and host address the same memory); null and the error text on failure.
 int* wait_flag();
-// Ends a call with an error if a wait of an earlier one ran out.
-int check_wait_flag(const char* who);
 
 // ---- clusters --------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
