@@ -479,6 +479,8 @@ __global__ void __launch_bounds__(kFewThreads) glu_few_kernel(const __grid_const
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
+    // A wait ran out: where the copies were all issued before, or the products, nobody above has waited for them; they land before the block ends.
+    if (*dead) tc::pause();
     if (warp == 2) {
         tc::fence_after_sync();
         tc::tmem_free(tmem, 2 * kAcc);
