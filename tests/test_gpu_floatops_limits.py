@@ -118,6 +118,33 @@ def test_gelu_far_below_zero(zkb, kind, n):
     near(dx, want, t, half_step(t) * want.abs() + 2.0 ** -16 * want.abs() + extra)
 
 
+# ---- gates at the ends of the type ---------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("kind,far", (("bf16", 1e30), ("bf16", 1e20), ("bf16", 1e13), ("bf16", 200.0), ("f16", 60000.0), ("f16", 200.0)))
+def test_glu_gates_far_from_zero(zkb, act, kind, far):
+    """act is the identity or zero there and its derivative one or zero, whatever the powers of g do on the way (f16: within its range)"""
+    code, t = TYPES[kind]
+    n, f = 130, 16
+    g = torch.full((n, 1), far, device="cuda").to(t)
+    g[1::2] *= -1
+    one, zero, ones = torch.ones(1, f, device="cuda", dtype=t), torch.zeros(1, f, device="cuda", dtype=t), torch.ones(n, 1, device="cuda", dtype=t)
+    for rows in (slice(0, 2), slice(0, n)):
+        x = g[rows]
+        m = x.shape[0]
+        h, gate, up = (torch.empty(m, f, device="cuda", dtype=t) for _ in range(3))
+        glu_call(zkb, code, act, x, one, one, h, gate, up)
+        assert torch.equal(gate, x.expand(m, f))
+        if far * far < torch.finfo(t).max:
+            assert torch.equal(h, (x.clamp(min=0) * x).expand(m, f))
+        dx = torch.empty(m, 1, device="cuda", dtype=t)
+        glu_back_call(zkb, code, act, ones[:m], one[:, :1], zero[:, :1], x, ones[:m], ones[:m], dx, None, None)
+        assert torch.equal(dx, (x > 0).to(t))
+        glu_back_call(zkb, code, act, ones[:m], zero[:, :1], one[:, :1], x, ones[:m], ones[:m], dx, None, None)
+        assert torch.equal(dx, x.clamp(min=0))
+
+
 # ---- calls beside one another ----------------------------------------------------------------------------------------------------------------------
 
 

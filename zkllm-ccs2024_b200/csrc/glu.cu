@@ -25,7 +25,8 @@ __device__ __forceinline__ float activate(float g, float* d) {
         // (1 + tanh k) / 2 = 1 / (1 + exp(-2k))
         const float k = 0.79788456080286536f * (g + 0.044715f * g * g * g);
         const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * k));
-        if (kDerivative) *d = s + 2.0f * g * s * (1.0f - s) * 0.79788456080286536f * (1.0f + 0.134145f * g * g);
+        // far out s (1 - s) is zero, and stays so beside a square that would pass 32 bits
+        if (kDerivative) *d = s + 2.0f * g * s * (1.0f - s) * 0.79788456080286536f * (1.0f + 0.134145f * fminf(g * g, 1e30f));
         return g * s;
     } else {
         if (kDerivative) *d = g > 0.0f ? 1.0f : 0.0f;
