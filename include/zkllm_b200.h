@@ -322,10 +322,11 @@ int zkb_softmax_decompose(const zkb_fr_t* d_X, const uint32_t* h_bs, unsigned K,
                           size_t N, void* stream);
 
 /* ---- the float side of a layer -------------------------------------------------------
- * The stages above work on fixed-point values; what those are made from - the norms' statistics, the turned queries and
- * keys, the feed-forward block that a fixed-point one is calibrated to, and the gradients that fit the weights before they
- * are fixed and committed - is float work.  These operators have no counterpart in the reference's C++ (its Python side
- * computes them: llama-rmsnorm.py:37-39, llama-self-attn.py:48-65, llama-ffn.py:16-19).
+ * The stages above work on fixed-point values.  These operators are the float pass of the same kind of layer and its gradients, for a
+ * host that runs, fits or checks a layer beside proving it.  One stage takes its input from them: rms-inv of zkllm-driver
+ * writes rmsnorm's side input with zkb_block_norm.  They have no counterpart in the reference's C++: its Python side
+ * computes the norms' statistics (llama-rmsnorm.py:37-39) and turns queries and keys (llama-self-attn.py:48-65), which its proven
+ * attention leaves out; the feed-forward block exists there in fixed point only, its activation a table (llama-ffn.py:16-19).
  *  - Tensors are device memory of the current device, of one type `dtype`; strides count elements, a row's values are
  *    consecutive and every stride and address may be any multiple of the element size.  16-byte alignment of addresses
  *    and strides is faster.  Host arrays and other devices' memory are refused.

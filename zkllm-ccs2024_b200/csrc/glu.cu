@@ -73,8 +73,8 @@ __device__ __forceinline__ void ungate(int act, float (&g)[N], float (&u)[N], co
 // the products (256 x 256 x 16 each) into one of two accumulators in tensor memory; warps 4 to 11 of both take their 128 rows of the other
 // accumulator out, so that a tile's epilogue runs beside the next tile's products.
 //
-// Measured: 2048 x 4096 x 11008 bf16, 238 to 299 us by the power the GPU has left (1.24 to 1.55 PFLOP/s; torch's two products alone 259 to
-// 265 us), the tensor pipe busy 87% of the time; gradients 595 us, 540 at best.  One block to a tile of 128 x 256 took 360 us; a switch over the
+// Measured: 2048 x 4096 x 11008 bf16, 300 to 310 us call after call under the power limit (1.2 PFLOP/s; torch's two products alone 259 to
+// 265 us), 238 for a single launch after idling, the tensor pipe busy 87% of the time; gradients 560 to 620 us, 520 at best.  One block to a tile of 128 x 256 took 360 us; a switch over the
 // activation inside the epilogue's loop 337; the gradients' two kinds of tiles in a launch each 10% more.  Fetching slices ahead into L2 only cost.
 //
 // The forms of a tile:
@@ -343,7 +343,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads) glu
 // block per SM takes a run of them, whole tiles or parts of tiles, through one ring that never drains, and leaves the sums of each
 // (part of a) tile in the workspace; glu_few_finish_kernel adds the parts of a tile, in order, and applies the activation.
 // Measured: one token through 4096 x 11008 bf16, 34 us with both kernels (5.3 TB/s of 6.56; reading the same boxes and nothing else 29 us); 48
-// tokens through 5120 x 13824 f16, 55 us (5.2 TB/s).
+// tokens through 5120 x 13824 f16, 55 to 57 us (5.1 TB/s).
 // Parts of a cluster that share a tile through distributed shared memory were measured before: no more than one such block ran on an
 // SM, and the ring of 72 KB that left to each read 4.0 TB/s.
 constexpr int kFewCols = 128, kFewThreads = 256;
@@ -757,8 +757,9 @@ template <class T, class Args>
 int product_launch(const Args& p, size_t tiles, cudaStream_t s) {
     const auto glu_product = glu_product_kernel<T, Args>;
     ZKB_CUDA(cudaFuncSetAttribute(glu_product, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kProductSmem));
-    // A plain launch, and no trigger in the kernel: small blocks of a successor that is launched beside it and waits for its end could take
-    // the SMs of a cluster that has no place yet, and neither would ever go on.
+    // A plain launch, and no trigger in the kernel.  While it took part in programmatic launches, a loop of gradient calls stalled twice; the
+    // cause is open (a successor starts only when every block has triggered, so it cannot have taken a cluster's place, and the warps that
+    // could part before instructions on tensor memory were mended at the same time), so it stays out of them.
     ZKB_LAUNCH(glu_product, 2 * (unsigned)std::min(tiles, (size_t)sm_count() / 2), kProductThreads, kProductSmem, s, p);
     return ZKB_OK;
 }
@@ -824,6 +825,8 @@ int glu_launch(const GluArgs& a, cudaStream_t s) {
     ZKB_TRY(before<T>(SplitArgs{}, {&x, &wg, &wu}, &scratch, s));
     int* const flag = tc::wait_flag();
     if (!flag) return ZKB_ERR_CUDA;
+    // The border: 4096 x 11008 bf16 takes 37 us for 16 tokens, 38 for 32, 41 for 64 and 44.5 for 128 with the tokens as the narrow operand, and
+    // 53 us for 129 as for 256 in the product kernel, whose tiles are 256 tokens high whatever they hold.
     if (a.tokens <= 16) return glu_few_launch<T, 16>(a, x, wg, wu, flag, &scratch, s);
     if (a.tokens <= 32) return glu_few_launch<T, 32>(a, x, wg, wu, flag, &scratch, s);
     if (a.tokens <= 64) return glu_few_launch<T, 64>(a, x, wg, wu, flag, &scratch, s);

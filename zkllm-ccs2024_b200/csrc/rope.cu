@@ -35,7 +35,7 @@ struct RopeArgs {
 // 32-bit product is off by 0.01 radians at position 131072) and only the fraction is rounded to 32.
 // P pairs make a unit of work, in 16-byte vectors where sizes, strides and addresses allow it, else one pair at a time.  A thread
 // keeps its unit and goes through the heads of the block's tokens, kAhead at a time so that their loads are in flight together.
-// Measured: 3 x 4097 tokens, 48 heads of 128, f32, 100 us (5.6 to 6.0 TB/s of 6.56); 2048 tokens, 64 heads, bf16, 18.5 us with the
+// Measured: 3 x 4097 tokens, 48 heads of 128, f32, 100 us (6.0 TB/s of 6.56), 107 with the host's call; 2048 tokens, 64 heads, bf16, 18.5 us with the
 // host's call.  Units dealt out anew for each vector (a division each) took 168 us for the first; four heads at a time needed 127
 // registers and took 29 us for the second; 128 threads and 4 tokens to a block beat 256 and 8 by 2 us there.
 template <class T, bool kWidePath, bool kInterleaved>
